@@ -172,6 +172,71 @@ SM_API int sm_attention_decode_noalloc(sm_ctx* ctx, const float* q, const float*
                                        float* out, const int* lens_dev, int B, int max_ctx, int n_heads, int n_kv,
                                        int head_dim);
 
+/* ---------------------------------------------------------------- 8-bit KV cache */
+/* A KV cache in 8 bits: int8 codes with one fp32 scale for every (slot, kv head,
+ * position), K and V each.  No counterpart in the reference, whose caches are
+ * fp32 (KvCacheEntry.cs:42-43): 4x (head_dim 128: 3.9x) less to keep and to read.
+ * The arrays are the caller's device memory; the struct only names them and may
+ * be reused for any number of calls.
+ *   k, v             int8  [max_seqs][n_kv][max_tokens][head_dim], 16-byte aligned
+ *   k_scale, v_scale float [max_seqs][n_kv][max_tokens]
+ * head_dim is 64 or 128.  A stored value is code * scale. */
+typedef struct sm_kv8 {
+  int8_t* k;
+  int8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int max_seqs;
+  int max_tokens;
+  int n_kv;
+  int head_dim;
+} sm_kv8;
+
+/* All four calls below take device pointers and run on the context's stream without
+ * synchronising; they can be captured into a CUDA graph.  A sequence id below 0 marks a padding row: nothing
+ * is read, and what the row would have written is left as it was.  A sequence id,
+ * position or length outside the cache is reported as SM_ERR_SHAPE by
+ * sm_ctx_device_status, and its row is treated like a padding row.  n_rows == 0 or
+ * B == 0 does nothing. */
+
+/* Quantise K and V rows into the cache: row i goes to position positions[i] of slot
+ * seq_ids[i].  k, v: row i at k + i * row_stride, [n_kv][head_dim] fp32 (row_stride
+ * in floats, >= n_kv * head_dim, so rows may sit inside a fused Q|K|V row).
+ * Per kv head: scale = max|x| / 127 in fp32, code = x / scale rounded to the
+ * nearest integer, ties to even (exactly, whatever the magnitudes); zeros give
+ * scale 0 and codes 0.  A head with an infinity or NaN gets scale NaN and codes 0,
+ * so it reads back as NaN.  Each (slot, position) at most once per call: what two
+ * rows with the same target leave in it is unspecified. */
+SM_API int sm_kv8_write(sm_ctx* ctx, const sm_kv8* cache, const float* k, const float* v, int64_t row_stride,
+                        const int* seq_ids, const int* positions, int n_rows);
+
+/* Read positions back (KvCacheEntry.GetKeys / GetValues, KvCacheEntry.cs:155-189, on
+ * device rows): row i of k and v = code * scale of position positions[i] of slot
+ * seq_ids[i].  Either of k and v may be NULL.  row_stride in floats. */
+SM_API int sm_kv8_read(sm_ctx* ctx, const sm_kv8* cache, const int* seq_ids, const int* positions, int n_rows,
+                       float* k, float* v, int64_t row_stride);
+
+/* sm_attention_decode over an 8-bit cache: one query row per sequence, row b attending
+ * to positions 0 .. lens[b] - 1 of slot seq_ids[b] (seq_ids NULL: slot b), with the
+ * reference's softmax (MathUtils.FastExp, MathUtils.cs:20-32).  q: row b at
+ * q + b * q_stride, [n_heads][head_dim]; out: [B][n_heads * head_dim].
+ * 0 <= lens[b] <= max_len <= max_tokens; a row of length 0 gives zeros.  max_len
+ * sizes the launch, so a graph captured with it serves every shorter length.
+ * n_heads is a multiple of n_kv, at most 16 q heads per kv head.  A NaN in q or in
+ * a visible scale makes the outputs that depend on it NaN. */
+SM_API int sm_attention_decode_kv8(sm_ctx* ctx, const sm_kv8* cache, const float* q, int64_t q_stride,
+                                   const int* seq_ids, const int* lens, int max_len, int B, int n_heads,
+                                   float* out);
+
+/* The same for a batch whose sequences share a prefix, which is kept and read once:
+ * row b attends to the first prefix_len positions of slot prefix_seq of `prefix`,
+ * then to positions 0 .. lens[b] - 1 of slot seq_ids[b] of `cache`.  The two caches
+ * may be the same; n_kv and head_dim have to agree.  prefix_len and prefix_seq are
+ * host values; lens may be 0 (a sequence that only has the prefix). */
+SM_API int sm_attention_shared_kv8(sm_ctx* ctx, const sm_kv8* prefix, int prefix_seq, int prefix_len,
+                                   const sm_kv8* cache, const float* q, int64_t q_stride, const int* seq_ids,
+                                   const int* lens, int max_len, int B, int n_heads, float* out);
+
 /* ---------------------------------------------------------------- model */
 /* ModelConfig fields used by the LLaMA path (ModelConfig.cs:14-136). */
 typedef struct sm_model_config {

@@ -40,6 +40,12 @@ class SamplingParams(C.Structure):
 SAMPLE_MAX_VOCAB = 53248
 
 
+class KV8(C.Structure):
+    """sm_kv8 (include/smallmind_cuda.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("max_seqs", C.c_int), ("max_tokens", C.c_int), ("n_kv", C.c_int), ("head_dim", C.c_int)]
+
+
 # name -> (restype, argtypes); every symbol declared in include/smallmind_cuda.h
 vp, i, i64, f, sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
 PP = C.POINTER(C.c_void_p)
@@ -68,6 +74,10 @@ SIGNATURES = {
     "sm_attention": (i, [vp, vp, vp, vp, vp, i, i, i, i, i, i]),
     "sm_attention_decode": (i, [vp, vp, vp, vp, vp, vp, i, i, i, i, i]),
     "sm_attention_decode_noalloc": (i, [vp, vp, vp, vp, vp, vp, i, i, i, i, i]),
+    "sm_kv8_write": (i, [vp, C.POINTER(KV8), vp, vp, i64, vp, vp, i]),
+    "sm_kv8_read": (i, [vp, C.POINTER(KV8), vp, vp, i, vp, vp, i64]),
+    "sm_attention_decode_kv8": (i, [vp, C.POINTER(KV8), vp, i64, vp, vp, i, i, i, vp]),
+    "sm_attention_shared_kv8": (i, [vp, C.POINTER(KV8), i, i, C.POINTER(KV8), vp, i64, vp, vp, i, i, i, vp]),
     "sm_model_create": (i, [vp, C.POINTER(ModelConfig), PP]),
     "sm_model_set_weight": (i, [vp, i, i, vp]),
     "sm_model_set_vector": (i, [vp, i, i, vp, sz]),

@@ -48,22 +48,10 @@ int ctx_view(sm_ctx* ctx, int* device, cudaStream_t* stream, int64_t** launches)
   *launches = &ctx->launches;
   return SM_OK;
 }
+int* ctx_status(sm_ctx* ctx) { return ctx ? ctx->dev_status : nullptr; }
 }  // namespace sm
 
 namespace {
-
-struct DeviceGuard {
-  int prev = -1;
-  explicit DeviceGuard(int dev) {
-    cudaGetDevice(&prev);
-    if (prev != dev) cudaSetDevice(dev);
-  }
-  ~DeviceGuard() {
-    int cur = -1;
-    cudaGetDevice(&cur);
-    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
-  }
-};
 
 bool valid_scheme(int s) {
   return s == SM_F32 || s == SM_Q8_0 || s == SM_Q4_0 || s == SM_Q4_1 || s == SM_Q5_0 || s == SM_Q4_K || s == SM_Q6_K;

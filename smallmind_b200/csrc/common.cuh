@@ -142,6 +142,22 @@ struct LaunchCounter {
 
 // capi.cu: device, stream and launch counter of a context
 int ctx_view(sm_ctx* ctx, int* device, cudaStream_t* stream, int64_t** launches);
+// capi.cu: the context's device-side status word (sm_ctx_device_status)
+int* ctx_status(sm_ctx* ctx);
+
+// Makes a device current for the lifetime of the guard.
+struct DeviceGuard {
+  int prev = -1;
+  explicit DeviceGuard(int dev) {
+    cudaGetDevice(&prev);
+    if (prev != dev) cudaSetDevice(dev);
+  }
+  ~DeviceGuard() {
+    int cur = -1;
+    cudaGetDevice(&cur);
+    if (prev >= 0 && cur != prev) cudaSetDevice(prev);
+  }
+};
 
 // ---------------------------------------------------------------- kernel entry points (host wrappers)
 // quant.cu
