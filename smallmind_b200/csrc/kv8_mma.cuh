@@ -1,0 +1,91 @@
+// Integer tensor-core pieces of the 8-bit KV cache's attention (mma.sync m16n8k32).
+//
+// The codes are the A operand as they are.  The fp32 side (q, or the softmax weights) enters as
+// fixed point: three bytes of an integer of up to 24 bits, one MMA per byte, whose exact int32
+// sums are put together in fp32.  So a product keeps fp32 accuracy and no code is converted.
+#pragma once
+#include <cstdint>
+
+#include "common.cuh"
+#include "mma_i8.cuh"
+
+namespace sm {
+
+// D += A B, A s8 codes [16 x 32], B the 8-bit digits of 8 columns [32 x 8]
+__device__ __forceinline__ void mma_s8u8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Bytes 0, 1 and 2 of four integers, each gathered into a word (integer 0 in the low byte).
+__device__ __forceinline__ void bytes3(uint32_t x0, uint32_t x1, uint32_t x2, uint32_t x3, uint32_t& lo, uint32_t& mid,
+                                       uint32_t& hi) {
+  const uint32_t a = __byte_perm(x0, x1, 0x5140), b = __byte_perm(x2, x3, 0x5140);
+  lo = __byte_perm(a, b, 0x5410);
+  mid = __byte_perm(a, b, 0x7632);
+  hi = __byte_perm(__byte_perm(x0, x1, 0x0062), __byte_perm(x2, x3, 0x0062), 0x5410);
+}
+
+// 4 x 4 bytes: w[i] holds columns 0..3 of row i; afterwards w[c] holds rows 0..3 of column c.
+__device__ __forceinline__ void transpose4(uint32_t& w0, uint32_t& w1, uint32_t& w2, uint32_t& w3) {
+  const uint32_t a = __byte_perm(w0, w1, 0x5140), b = __byte_perm(w2, w3, 0x5140);
+  const uint32_t c = __byte_perm(w0, w1, 0x7362), d = __byte_perm(w2, w3, 0x7362);
+  w0 = __byte_perm(a, b, 0x5410);
+  w1 = __byte_perm(a, b, 0x7632);
+  w2 = __byte_perm(c, d, 0x5410);
+  w3 = __byte_perm(c, d, 0x7632);
+}
+
+// hi * 2^16 + mid * 2^8 + lo of three digit sums; join3_small: |mid| and |lo| < 2^22
+__device__ __forceinline__ float join3_small(int hi, int mid, int lo) {
+  return fmaf((float)hi, 65536.f, (float)(mid * 256 + lo));
+}
+__device__ __forceinline__ float join3(int hi, int mid, int lo) {
+  return fmaf((float)hi, 65536.f, fmaf((float)mid, 256.f, (float)lo));
+}
+
+// Larger of the two, NaN if either is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// The softmax weight of x = score - maximum: (12 + 6x + x^2) / (12 - 6x + x^2) at max(x, -87.3).
+// The reciprocal is the hardware's (1 ulp); a NaN stays one.
+__device__ __forceinline__ float kv8_weight(float x) {
+  const float c = max_nan(x, -87.3f);
+  const float a = fmaf(c, c, 12.f);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(-6.f, c, a)));
+  return fmaf(6.f, c, a) * r;
+}
+
+// 16 / 8 / 4 bytes of codes that are read once
+__device__ __forceinline__ uint4 ld_codes16(const int8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_codes8(const int8_t* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_codes4(const int8_t* p) {
+  uint32_t v;
+  asm volatile("ld.global.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+
+}  // namespace sm
