@@ -7,6 +7,7 @@
 // partial results against a running maximum cannot be rescaled: the exact maximum comes
 // first and the weights are formed against it.
 #include <cooperative_groups.h>
+#include <cstdlib>
 
 #include "kv8.cuh"
 #include "kv8_mma.cuh"
@@ -89,43 +90,44 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_kernel(Kv8Attn a) {
     a.out[((int64_t)b * a.n_heads + h) * HD + threadIdx.x] = total > 0 ? __fdiv_rn(acc, sum) : 0.f;
 }
 
-// ---------------------------------------------------------------- decode: one cluster per (sequence, kv head)
+// ---------------------------------------------------------------- pieces of the decode kernels
 //
-// The keys are split over the cluster's CTAs, 16 keys x 8 query heads an MMA tile:
-//   1. scores: K codes go from global memory into A fragments as they lie (a lane takes 16
-//      neighbouring bytes of a row; q's digits, built once, are in the matching order) and the
-//      scores stay in shared memory, GP floats a key;
-//   2. the exact maximum of each head over the cluster (distributed shared memory);
-//   3. weights e and P = e * v_scale in 23-bit fixed point against the slice's largest v_scale;
-//      the three digits replace the scores in place, in B-fragment order;
-//   4. out += P V: V codes become A fragments (row = dim, k = key) by 4 x 4 byte transposes;
-//   5. each CTA joins its warps' sums, each rank its share of the outputs over the cluster.
-// Bound by HBM at length (one pass over the codes), by the chain of phases when short.
+// Keys are taken in blocks of 32, a warp each:
+//   scores  two 16-key x 8-head MMA tiles.  K codes go from global memory into A fragments as they
+//           lie: a lane takes 16 neighbouring bytes of a row, and q's digits, built once, are in
+//           the matching order.  A lane's four rows are the keys whose scores the P side wants
+//           side by side.  Scores are kept without the head's positive factor, which a maximum
+//           does not need;
+//   P V     weights e, and P = e * v_scale in 23-bit fixed point against the largest v_scale of
+//           the warp's keys, in the registers that the MMA wants them in; V codes are made
+//           fragments by 4 x 4 byte transposes.  With up to 4 heads the three digits of all of
+//           them are rows of one A operand; with more, a digit is a B operand of 8 heads.
 constexpr int DT = 256;
 constexpr int DW = DT / 32;
 
 template <int HD, int GP>
 struct Tile {
+  static constexpr bool PA = GP == 4;           // P's digits as the A operand
   static constexpr int NT = GP > 8 ? 2 : 1;     // column tiles of 8 heads
   static constexpr int CP = GP > 8 ? 8 : GP;    // heads a tile keeps
-  static constexpr int KI = HD / 32;            // MMA steps of a score
-  static constexpr int LD = HD / 64;            // 16-byte loads of a row a lane
-  static constexpr int DS = (HD / 64) * NT;     // warps that split the dims of one key block
+  static constexpr int ZB = 32 * CP;            // scores of a block and column tile
+  static constexpr int DS = HD == 128 && GP == 16 ? 2 : 1;  // warps that split the dims of a key block
   static constexpr int TW = DW / DS;            // warps that split the keys
   static constexpr int DP = HD / DS;            // dims a warp
-  static constexpr int MT = DP / 16;            // 16-row tiles of dims
   static constexpr int VB = DP / 8;             // bytes of a V row a lane
-  // shared memory, in floats: scores | per-CTA results for the cluster
-  static constexpr int PART = TW * GP * HD;     // the warps' sums take the scores' place
-  static constexpr int TAIL = GP * HD + 2 * GP;
-  static __host__ __device__ size_t smem_floats(int cap) {
-    const int s = cap * GP;
-    return (size_t)(s > PART ? s : PART) + TAIL;
-  }
+  // accumulator tiles: PA one for each byte of a lane (8 dims), else 16 dims x (heads, digits)
+  static constexpr int MT = PA ? VB : DP / 16;
+  static constexpr int MD = PA ? 1 : 3 * NT;
+  static constexpr int PART = TW * GP * HD;     // floats of the warps' sums
 };
 
-// q of one kv head's group as digits in B-fragment order; `unit` gets 2^e / sqrt(HD) of this lane's
-// column head (lane / 4), the factor of its digit sums (NaN where q is not finite).
+// Scores of a block lie as [head][t][8]: the scores of keys t + 4 i, i = 0..7, in a row.
+// A lane's rows of the score tiles are keys krow(g) + 4 c, c = 0..3: half of such a row.
+__device__ __forceinline__ int krow(int g) { return (g & 3) + 16 * (g >> 2); }
+__device__ __forceinline__ int zpos(int head, int g) { return head * 32 + (g & 3) * 8 + (g >> 2) * 4; }
+
+// q of one kv head's group as digits in B-fragment order; `unit` gets 2^(e - 22) / sqrt(HD) of this
+// lane's column head (lane / 4), the factor of its digit sums (NaN where q is not finite).
 template <int HD, int GP>
 __device__ __forceinline__ void load_q(const float* q, int G, int lane, uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
                                        float (&unit)[Tile<HD, GP>::NT]) {
@@ -137,13 +139,9 @@ __device__ __forceinline__ void load_q(const float* q, int G, int lane, uint32_t
     float x[HD / 4];
     float peak = 0.f;
 #pragma unroll
-    for (int l = 0; l < T::LD; ++l)
+    for (int i = 0; i < HD / 4; ++i) x[i] = h < G ? q[h * HD + (i / 16) * 64 + 16 * t + i % 16] : 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float v = h < G ? q[h * HD + l * 64 + 16 * t + i] : 0.f;
-        x[l * 16 + i] = v;
-        peak = max_nan(peak, fabsf(v));
-      }
+    for (int i = 0; i < HD / 4; ++i) peak = max_nan(peak, fabsf(x[i]));
     peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
     peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
     const bool ok = peak < INFINITY;
@@ -162,8 +160,246 @@ __device__ __forceinline__ void load_q(const float* q, int G, int lane, uint32_t
   }
 }
 
+// K codes and scales of a block, as a lane holds them: rows krow(g) + 4 c, bytes 16 t .. of each 64.
+// Rows at or past n repeat row n - 1, which leaves a maximum as it is.
+template <int HD>
+struct KBlock {
+  uint32_t w[4][HD / 64][4];
+  float s[4];
+  __device__ __forceinline__ void load(const int8_t* kp, const float* ksp, int row, int n, int g, int t) {
+    const int r = row + krow(g);
+    const int8_t* p = kp + (int64_t)r * HD + 16 * t;
+    if (row + 32 <= n) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int l = 0; l < HD / 64; ++l) ld_codes(p + 4 * c * HD + l * 64, w[c][l]);
+        s[c] = __ldg(ksp + r + 4 * c);
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int o = min(4 * c, n - 1 - r);
+#pragma unroll
+        for (int l = 0; l < HD / 64; ++l) ld_codes(p + o * HD + l * 64, w[c][l]);
+        s[c] = __ldg(ksp + r + o);
+      }
+    }
+  }
+};
+
+// Scores of a block: to z ([NT] planes `plane` floats apart), and this lane's running maxima of columns 2t, 2t + 1.
 template <int HD, int GP>
-__global__ void __launch_bounds__(DT, (HD == 128 && GP == 16) ? 1 : 2) decode_kv8_kernel(Kv8Attn a, int cap) {
+__device__ __forceinline__ void score_block(const KBlock<HD>& k, const uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
+                                            int g, int t, float* z, int64_t plane,
+                                            float (&mx)[Tile<HD, GP>::NT][2]) {
+  using T = Tile<HD, GP>;
+#pragma unroll
+  for (int nt = 0; nt < T::NT; ++nt) {
+    float s[4][2];  // key krow(g) + 4 c, column 2t + i
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      int d[3][4] = {};
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) {
+        const uint32_t a0 = k.w[2 * m][i >> 1][2 * (i & 1)], a2 = k.w[2 * m][i >> 1][2 * (i & 1) + 1];
+        const uint32_t a1 = k.w[2 * m + 1][i >> 1][2 * (i & 1)], a3 = k.w[2 * m + 1][i >> 1][2 * (i & 1) + 1];
+        mma_s8u8(d[0], a0, a1, a2, a3, qd[nt][i][0][0], qd[nt][i][0][1]);
+        mma_s8u8(d[1], a0, a1, a2, a3, qd[nt][i][1][0], qd[nt][i][1][1]);
+        mma_s8s8(d[2], a0, a1, a2, a3, qd[nt][i][2][0], qd[nt][i][2][1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[2 * m + (i >> 1)][i & 1] = join3_small(d[2][i], d[1][i], d[0][i]) * k.s[2 * m + (i >> 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      mx[nt][i] = fmaxf(mx[nt][i], fmaxf(fmaxf(s[0][i], s[1][i]), fmaxf(s[2][i], s[3][i])));
+      if (2 * t < T::CP)
+        *(float4*)(z + nt * plane + zpos(2 * t + i, g)) = make_float4(s[0][i], s[1][i], s[2][i], s[3][i]);
+    }
+  }
+}
+
+// Maxima of a warp's columns (lanes g of one t merged) into to[GP]
+template <int HD, int GP>
+__device__ __forceinline__ void warp_maxima(const float (&mx)[Tile<HD, GP>::NT][2], int g, int t, float* to) {
+#pragma unroll
+  for (int nt = 0; nt < Tile<HD, GP>::NT; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float m = mx[nt][c];
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+      if (g == 0 && 2 * t < Tile<HD, GP>::CP) to[nt * 8 + 2 * t + c] = m;
+    }
+}
+
+// V codes of a block: keys t + 4 i, VB dims of each; and the scale of key `lane` (0 past the end).
+template <int HD, int GP>
+struct VBlock {
+  using T = Tile<HD, GP>;
+  uint32_t w[8][T::VB / 4];
+  float s;
+  __device__ __forceinline__ void load(const int8_t* vp, const float* vsp, int row, int n, int lane, int d0) {
+    const int g = lane >> 2, t = lane & 3;
+    const int8_t* p = vp + (int64_t)(row + t) * HD + d0 + g * T::VB;
+    if (row + 32 <= n) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ld_codes(p + 4 * i * HD, w[i]);
+      s = __ldg(vsp + row + lane);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ld_codes(p + min(4 * i, n - 1 - row - t) * HD, w[i]);
+      s = row + lane < n ? __ldg(vsp + row + lane) : 0.f;
+    }
+  }
+};
+
+// What a warp accumulates of P V, and how P is formed.
+template <int HD, int GP>
+struct PVSum {
+  using T = Tile<HD, GP>;
+  float m[T::NT], unit[T::NT], esum[T::NT];  // of this lane's head: factored maximum, factor, sum of weights
+  float mult, back;                          // fixed point: e = 1 at scale vmax is 2^23 - 8
+  int acc[T::MD][T::MT][4];
+
+  // A lane's head is column g of each tile; with P as A both halves of the rows hold heads 0..3.
+  static __device__ __forceinline__ int column(int g) { return T::PA ? g & 3 : g; }
+
+  // Scales under 1e-30 keep the resolution of 1e-30, so that neither factor overflows.
+  __device__ __forceinline__ void start(float vmax, const float (&max_of)[T::NT], const float (&unit_of)[T::NT]) {
+    vmax = max_nan(vmax, 1e-30f);
+    mult = 8388600.f / vmax;
+    back = vmax * (1.f / 8388600.f);
+#pragma unroll
+    for (int nt = 0; nt < T::NT; ++nt) unit[nt] = unit_of[nt], m[nt] = max_of[nt] * unit_of[nt], esum[nt] = 0.f;
+#pragma unroll
+    for (int i = 0; i < T::MD; ++i)
+#pragma unroll
+      for (int c = 0; c < T::MT; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][c][e] = 0;
+  }
+
+  // zv: the lane's 8 scores of each tile; keys: how many of the block's 32 exist.  v is used up.
+  __device__ __forceinline__ void add(VBlock<HD, GP>& v, const float (&zv)[T::NT][8], int keys, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    const float vsm = v.s * mult;
+    uint32_t dg[T::NT][3][2];
+#pragma unroll
+    for (int nt = 0; nt < T::NT; ++nt) {
+      float e[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = kv8_weight(fmaf(zv[nt][i], unit[nt], -m[nt]));
+      if (keys < 32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (t + 4 * i >= keys) e[i] = 0.f;
+      }
+      float part = 0.f;
+      uint32_t p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        part += e[i];
+        // e * scale lies in [0, 2^23): added to 2^23 it is the mantissa, rounded
+        p[i] = __float_as_uint(fmaf(e[i], __shfl_sync(0xffffffffu, vsm, t + 4 * i), 8388608.f));
+      }
+      esum[nt] += part;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        bytes3(p[4 * half], p[4 * half + 1], p[4 * half + 2], p[4 * half + 3], dg[nt][0][half], dg[nt][1][half],
+               dg[nt][2][half]);
+    }
+#pragma unroll
+    for (int c = 0; c < T::VB / 4; ++c) {
+      transpose4(v.w[0][c], v.w[1][c], v.w[2][c], v.w[3][c]);
+      transpose4(v.w[4][c], v.w[5][c], v.w[6][c], v.w[7][c]);
+    }
+    if constexpr (T::PA) {
+      // rows: digit 0 of heads 0..3, digit 1, digit 2, zeros
+      const uint32_t a0 = g < 4 ? dg[0][0][0] : dg[0][1][0], a2 = g < 4 ? dg[0][0][1] : dg[0][1][1];
+      const uint32_t a1 = g < 4 ? dg[0][2][0] : 0u, a3 = g < 4 ? dg[0][2][1] : 0u;
+#pragma unroll
+      for (int c = 0; c < T::MT; ++c)
+        mma_u8s8_acc(acc[0][c], a0, a1, a2, a3, v.w[c & 3][c >> 2], v.w[4 + (c & 3)][c >> 2]);
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < T::MT; ++mt) {
+        // the lane's bytes 2 mt and 2 mt + 1 are rows g and g + 8 of the tile
+        const int c = mt >> 1, o = (mt & 1) * 2;
+#pragma unroll
+        for (int i = 0; i < 3 * T::NT; ++i)
+          mma_s8u8(acc[i][mt], v.w[o][c], v.w[o + 1][c], v.w[4 + o][c], v.w[4 + o + 1][c], dg[i / 3][i % 3][0],
+                   dg[i / 3][i % 3][1]);
+      }
+    }
+  }
+
+  // The warp's sums to to[GP][HD], its weights' to sums[GP] (of the warps at d0 == 0).
+  __device__ __forceinline__ void store(float* to, float* sums, int lane, int d0) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < T::NT; ++nt) {
+      esum[nt] += __shfl_xor_sync(0xffffffffu, esum[nt], 1);
+      esum[nt] += __shfl_xor_sync(0xffffffffu, esum[nt], 2);
+      if (t == 0 && g < T::CP && d0 == 0) sums[nt * 8 + g] = esum[nt];
+    }
+    if constexpr (T::PA) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float o[T::MT];
+#pragma unroll
+        for (int c = 0; c < T::MT; ++c)
+          o[c] = join3(acc[0][c][2 + i], __shfl_xor_sync(0xffffffffu, acc[0][c][i], 16), acc[0][c][i]) * back;
+        if (g < 4) {
+#pragma unroll
+          for (int c = 0; c < T::MT; c += 4)
+            *(float4*)(to + g * HD + (2 * t + i) * T::VB + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < T::NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < T::MT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float* p = to + (nt * 8 + 2 * t + i) * HD + d0 + g * T::VB + 2 * mt;
+            *(float2*)p = make_float2(
+                join3(acc[3 * nt + 2][mt][i], acc[3 * nt + 1][mt][i], acc[3 * nt][mt][i]) * back,
+                join3(acc[3 * nt + 2][mt][i + 2], acc[3 * nt + 1][mt][i + 2], acc[3 * nt][mt][i + 2]) * back);
+          }
+    }
+  }
+};
+
+// Row b's slot and length; false where there is nothing to do (padding) or the row is out of range.
+__device__ __forceinline__ bool row_keys(const Kv8Attn& a, int b, int& slot, int& len) {
+  slot = a.seq_ids ? a.seq_ids[b] : b;
+  if (slot < 0) return false;
+  len = a.lens[b];
+  if (slot >= a.c.slots || len < 0 || len > a.max_len) {
+    if (threadIdx.x == 0) atomicExch(a.status, SM_ERR_SHAPE);
+    return false;
+  }
+  return true;
+}
+
+// ---------------------------------------------------------------- decode, short: one cluster per (sequence, kv head)
+//
+// One launch: the keys are split over the cluster's CTAs, the scores stay in shared memory, and the
+// exact maximum and the sums travel through distributed shared memory.  Bound by its chain of phases.
+template <int HD, int GP>
+struct ClusterSmem {
+  using T = Tile<HD, GP>;
+  static constexpr int TAIL = GP * HD + 2 * GP;  // this CTA's sums, maxima and weights for the cluster
+  static __host__ __device__ int64_t score_floats(int cap) { return cap * GP > T::PART ? cap * GP : T::PART; }
+  static size_t bytes(int cap) { return (score_floats(cap) + TAIL) * sizeof(float); }
+};
+
+template <int HD, int GP>
+__global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1) decode_kv8_kernel(Kv8Attn a, int cap) {
   using T = Tile<HD, GP>;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -171,27 +407,21 @@ __global__ void __launch_bounds__(DT, (HD == 128 && GP == 16) ? 1 : 2) decode_kv
   const int gk = blockIdx.y, b = blockIdx.z;
   const int G = a.n_heads / a.c.n_kv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  extern __shared__ __align__(16) float sm_[];
-  float* z = sm_;                                             // [NT][cap][CP]
-  float* pacc = sm_ + (T::smem_floats(cap) - T::TAIL);        // [GP][HD] this CTA's sums
-  float* stat = pacc + GP * HD;                               // [GP] maximum, [GP] sum of weights
+  extern __shared__ __align__(16) float z[];                    // [NT][cap / 32] score blocks
+  float* pacc = z + ClusterSmem<HD, GP>::score_floats(cap);     // [GP][HD] this CTA's sums
+  float* stat = pacc + GP * HD;                                 // [GP] maximum, [GP] sum of weights
   __shared__ float wred[DW][GP], vred[DW], gmax[GP];
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int slot = a.seq_ids ? a.seq_ids[b] : b;
-  if (slot < 0) return;
-  const int len = a.lens[b];
+  int slot, len;
+  if (!row_keys(a, b, slot, len)) return;
   float* out = a.out + ((int64_t)b * a.n_heads + gk * G) * HD;
-  if (slot >= a.c.slots || len < 0 || len > a.max_len) {
-    if (tid == 0) atomicExch(a.status, SM_ERR_SHAPE);
-    return;
-  }
   if (len == 0) {
     if (rank == 0)
       for (int i = tid; i < G * HD; i += DT) out[i] = 0.f;
     return;
   }
-  // this CTA's keys: whole blocks of 32
+  // this CTA's keys: whole blocks
   const int per = ((len + CL - 1) / CL + 31) & ~31;
   const int j0 = min(len, rank * per), n = min(len - j0, per);
   const int64_t row0 = a.c.at(slot, gk, j0);
@@ -199,98 +429,26 @@ __global__ void __launch_bounds__(DT, (HD == 128 && GP == 16) ? 1 : 2) decode_kv
   const int8_t* vp = a.c.v + row0 * HD;
   const float* ksp = a.c.ks + row0;
   const float* vsp = a.c.vs + row0;
+  const int64_t plane = (int64_t)cap * T::CP;
 
-  // ---- 1. scores
-  const int tiles = (n + 15) >> 4;
-  uint4 ka[T::LD], kb[T::LD];
-  float sa = 0.f, sb = 0.f;
-  auto load_k = [&](int tile) {
-    const int ra = min(tile * 16 + g, n - 1), rb = min(tile * 16 + 8 + g, n - 1);
-#pragma unroll
-    for (int l = 0; l < T::LD; ++l) {
-      ka[l] = ld_codes16(kp + (int64_t)ra * HD + l * 64 + 16 * t);
-      kb[l] = ld_codes16(kp + (int64_t)rb * HD + l * 64 + 16 * t);
-    }
-    sa = __ldg(ksp + ra);
-    sb = __ldg(ksp + rb);
-  };
-  if (warp < tiles) load_k(warp);
+  KBlock<HD> k;
+  if (32 * warp < n) k.load(kp, ksp, 32 * warp, n, g, t);
   float vmax = 0.f;
   for (int j = tid; j < n; j += DT) vmax = max_nan(vmax, __ldg(vsp + j));
-  uint32_t qd[T::NT][T::KI][3][2];
-  float unit[T::NT];
+  uint32_t qd[T::NT][HD / 32][3][2];
+  float unit[T::NT], mx[T::NT][2];
   load_q<HD, GP>(a.q + (int64_t)b * a.q_stride + (int64_t)gk * G * HD, G, lane, qd, unit);
-  float u[T::NT][2], mx[T::NT][2];  // factors and running maxima of this lane's score columns 2t, 2t + 1
 #pragma unroll
-  for (int nt = 0; nt < T::NT; ++nt)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      u[nt][c] = __shfl_sync(0xffffffffu, unit[nt], (2 * t + c) * 4);
-      mx[nt][c] = -INFINITY;
-    }
-  for (int tile = warp; tile < tiles; tile += DW) {
-    uint4 ca[T::LD], cb[T::LD];
-#pragma unroll
-    for (int l = 0; l < T::LD; ++l) ca[l] = ka[l], cb[l] = kb[l];
-    const float fa = sa, fb = sb;
-    if (tile + DW < tiles) load_k(tile + DW);
-    const int r = tile * 16 + g;
-#pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt) {
-      int d[3][4] = {};
-#pragma unroll
-      for (int l = 0; l < T::LD; ++l) {
-        const uint32_t* wa = (const uint32_t*)&ca[l];
-        const uint32_t* wb = (const uint32_t*)&cb[l];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const auto& q3 = qd[nt][2 * l + i];
-          mma_s8u8(d[0], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], q3[0][0], q3[0][1]);
-          mma_s8u8(d[1], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], q3[1][0], q3[1][1]);
-          mma_s8s8(d[2], wa[2 * i], wb[2 * i], wa[2 * i + 1], wb[2 * i + 1], q3[2][0], q3[2][1]);
-        }
-      }
-      float s[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = join3_small(d[2][i], d[1][i], d[0][i]) * (u[nt][i & 1] * (i < 2 ? fa : fb));
-      if (r < n) mx[nt][0] = fmaxf(mx[nt][0], s[0]), mx[nt][1] = fmaxf(mx[nt][1], s[1]);
-      if (r + 8 < n) mx[nt][0] = fmaxf(mx[nt][0], s[2]), mx[nt][1] = fmaxf(mx[nt][1], s[3]);
-      if (2 * t < T::CP) {
-        float* to = z + ((int64_t)nt * cap + r) * T::CP + 2 * t;
-        *(float2*)to = make_float2(s[0], s[1]);
-        *(float2*)(to + 8 * T::CP) = make_float2(s[2], s[3]);
-      }
-    }
+  for (int nt = 0; nt < T::NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
+  for (int row = 32 * warp; row < n; row += 32 * DW) {
+    score_block<HD, GP>(k, qd, g, t, z + (row >> 5) * T::ZB, plane, mx);
+    if (row + 32 * DW < n) k.load(kp, ksp, row + 32 * DW, n, g, t);
   }
   // the warp's first V block travels while the maxima are exchanged
   const int tw = warp / T::DS, d0 = (warp % T::DS) * T::DP;
-  const int blocks = (n + 31) >> 5;
-  uint32_t vw[8][T::VB / 4];
-  auto load_v = [&](int blk) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int8_t* p = vp + (int64_t)min(blk * 32 + t + 4 * i, n - 1) * HD + d0 + g * T::VB;
-      if constexpr (T::VB == 8) {
-        const uint2 v = ld_codes8(p);
-        vw[i][0] = v.x, vw[i][1] = v.y;
-      } else {
-        vw[i][0] = ld_codes4(p);
-      }
-    }
-  };
-  if (tw < blocks) load_v(tw);
-
-  // ---- 2. maxima: warps, CTA, cluster
-#pragma unroll
-  for (int nt = 0; nt < T::NT; ++nt)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      float m = mx[nt][c];
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-      if (g == 0 && 2 * t < T::CP) wred[warp][nt * 8 + 2 * t + c] = m;
-    }
+  VBlock<HD, GP> v;
+  if (32 * tw < n) v.load(vp, vsp, 32 * tw, n, lane, d0);
+  warp_maxima<HD, GP>(mx, g, t, wred[warp]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) vmax = max_nan(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
   if (lane == 0) vred[warp] = vmax;
@@ -298,11 +456,11 @@ __global__ void __launch_bounds__(DT, (HD == 128 && GP == 16) ? 1 : 2) decode_kv
   if (tid < GP) {
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < DW; ++w) m = fmaxf(m, wred[w][tid]);
+    for (int i = 0; i < DW; ++i) m = fmaxf(m, wred[i][tid]);
     stat[tid] = m;
   }
 #pragma unroll
-  for (int w = 0; w < DW; ++w) vmax = max_nan(vmax, vred[w]);
+  for (int i = 0; i < DW; ++i) vmax = max_nan(vmax, vred[i]);
   cluster.sync();
   if (tid < GP) {
     float m = -INFINITY;
@@ -311,120 +469,44 @@ __global__ void __launch_bounds__(DT, (HD == 128 && GP == 16) ? 1 : 2) decode_kv
   }
   __syncthreads();
 
-  // ---- 3. weights; P in fixed point: e = 1 at the largest scale is 2^23 - 8 (scales under 1e-30 keep the
-  // resolution of 1e-30, so that neither factor overflows)
-  vmax = max_nan(vmax, 1e-30f);
-  const float mult = 8388600.f / vmax;
-  float esum[T::NT];
-#pragma unroll
-  for (int nt = 0; nt < T::NT; ++nt) esum[nt] = 0.f;
-  const int col = g < T::CP ? g : 0;
-  for (int blk = warp; blk < blocks; blk += DW) {
-    float vs[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) vs[i] = __ldg(vsp + min(blk * 32 + t + 4 * i, n - 1)) * mult;
-#pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt) {
-      float* zb = z + ((int64_t)nt * cap + blk * 32) * T::CP;
-      const float m = gmax[nt * 8 + col];
-      uint32_t p[8];
-      float part = 0.f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = t + 4 * i;
-        float e = kv8_weight(zb[j * T::CP + col] - m);
-        if (blk * 32 + j >= n) e = 0.f;
-        part += e;
-        // e * vs lies in [0, 2^23): added to 2^23 it is the mantissa, rounded
-        p[i] = __float_as_uint(fmaf(e, vs[i], 8388608.f));
-      }
-      esum[nt] += part;
-      uint32_t dg[3][2];
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-        bytes3(p[4 * half], p[4 * half + 1], p[4 * half + 2], p[4 * half + 3], dg[0][half], dg[1][half], dg[2][half]);
-      __syncwarp();
-      if (g < T::CP) {
-        uint32_t* to = (uint32_t*)zb + lane;
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-          to[(2 * i) * 4 * T::CP] = dg[i][0];
-          to[(2 * i + 1) * 4 * T::CP] = dg[i][1];
-        }
-      }
-    }
-  }
+  PVSum<HD, GP> pv;
+  const int col = pv.column(g);
+  float max_of[T::NT];
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) {
-    esum[nt] += __shfl_xor_sync(0xffffffffu, esum[nt], 1);
-    esum[nt] += __shfl_xor_sync(0xffffffffu, esum[nt], 2);
-    if (t == 0 && g < T::CP) wred[warp][nt * 8 + g] = esum[nt];
+    unit[nt] = __shfl_sync(0xffffffffu, unit[nt], col * 4);
+    max_of[nt] = gmax[nt * 8 + col];
   }
+  pv.start(vmax, max_of, unit);
+  for (int row = 32 * tw; row < n; row += 32 * T::TW) {
+    float zv[T::NT][8];
+#pragma unroll
+    for (int nt = 0; nt < T::NT; ++nt) {
+      const float4* zb = (const float4*)(z + nt * plane + (row >> 5) * T::ZB + col * 32 + t * 8);
+      *(float4*)&zv[nt][0] = zb[0];
+      *(float4*)&zv[nt][4] = zb[1];
+    }
+    pv.add(v, zv, n - row, lane);
+    if (row + 32 * T::TW < n) v.load(vp, vsp, row + 32 * T::TW, n, lane, d0);
+  }
+  __syncthreads();  // the scores are read
+  float* part = z;  // [TW][GP][HD]
+  pv.store(part + tw * GP * HD, wred[tw], lane, d0);
   __syncthreads();
   if (tid < GP) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < DW; ++w) s += wred[w][tid];
+    for (int i = 0; i < T::TW; ++i) s += wred[i][tid];
     stat[GP + tid] = s;
   }
-
-  // ---- 4. sums of P V
-  int acc[T::NT][T::MT][3][4] = {};
-  for (int blk = tw; blk < blocks; blk += T::TW) {
-    uint32_t w[8][T::VB / 4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int c = 0; c < T::VB / 4; ++c) w[i][c] = vw[i][c];
-    if (blk + T::TW < blocks) load_v(blk + T::TW);
-    uint32_t dg[T::NT][3][2];
-#pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt) {
-      const uint32_t* from = (const uint32_t*)(z + ((int64_t)nt * cap + blk * 32) * T::CP) + lane;
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-#pragma unroll
-        for (int half = 0; half < 2; ++half) dg[nt][i][half] = g < T::CP ? from[(2 * i + half) * 4 * T::CP] : 0u;
-    }
-#pragma unroll
-    for (int c = 0; c < T::VB / 4; ++c) {
-      transpose4(w[0][c], w[1][c], w[2][c], w[3][c]);
-      transpose4(w[4][c], w[5][c], w[6][c], w[7][c]);
-    }
-#pragma unroll
-    for (int mt = 0; mt < T::MT; ++mt) {
-      // lane's dims 2 mt, 2 mt + 1 are rows g and g + 8 of the tile
-      const int c = mt >> 1, o = (mt & 1) * 2;
-#pragma unroll
-      for (int nt = 0; nt < T::NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 3; ++i)
-          mma_s8u8(acc[nt][mt][i], w[o][c], w[o + 1][c], w[4 + o][c], w[4 + o + 1][c], dg[nt][i][0], dg[nt][i][1]);
-    }
-  }
-  __syncthreads();  // the digits are read
-  float* part = sm_;  // [TW][GP][HD]
-  const float back = vmax * (1.f / 8388600.f);
-#pragma unroll
-  for (int nt = 0; nt < T::NT; ++nt)
-#pragma unroll
-    for (int mt = 0; mt < T::MT; ++mt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int h = nt * 8 + 2 * t + (i & 1), d = d0 + g * T::VB + 2 * mt + (i >> 1);
-        if (h < G)
-          part[(tw * GP + h) * HD + d] =
-              join3(acc[nt][mt][2][i], acc[nt][mt][1][i], acc[nt][mt][0][i]) * back;
-      }
-  __syncthreads();
   for (int i = tid; i < G * HD; i += DT) {
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < T::TW; ++w) s += part[w * GP * HD + i];
+    for (int r = 0; r < T::TW; ++r) s += part[r * GP * HD + i];
     pacc[i] = s;
   }
   cluster.sync();
-  // ---- 5. each rank its share of the outputs
+  // each rank its share of the outputs
   for (int i = rank * DT + tid; i < G * HD; i += CL * DT) {
     float s = 0.f, total = 0.f;
     for (int r = 0; r < CL; ++r) {
@@ -434,6 +516,172 @@ __global__ void __launch_bounds__(DT, (HD == 128 && GP == 16) ? 1 : 2) decode_kv
     out[i] = __fdiv_rn(s, total);
   }
   cluster.sync();  // no CTA's shared memory goes before the others have read it
+}
+
+// ---------------------------------------------------------------- decode, long: scores, P V and join as three launches
+//
+// Flat grids over chunks of keys, so that nothing waits inside a kernel: the scores of a chunk go to
+// global memory with the chunk's maxima (and its largest V scale), the second kernel reads them back
+// against the maximum over the chunks, the third joins the chunks' sums.  The scores add GP * 8 bytes
+// to the 2 * HD + 8 of a key and mostly stay in L2.  Bound by HBM.
+struct Kv8Split {
+  Kv8Attn a;
+  int chunk, n_chunks;  // keys of a chunk (whole blocks); chunks that max_len makes
+  float* z;             // [B][n_kv][NT][blocks] score blocks
+  float* stat;          // [B][n_kv][n_chunks][GP + 1] maxima, largest V scale
+  float* pacc;          // [B][n_kv][n_chunks][GP][HD]
+  float* psum;          // [B][n_kv][n_chunks][GP]
+};
+
+template <int HD, int GP>
+__global__ void __launch_bounds__(DT, GP == 16 ? 1 : 2) split_scores_kernel(Kv8Split s) {
+  using T = Tile<HD, GP>;
+  const Kv8Attn& a = s.a;
+  const int ch = blockIdx.x, gk = blockIdx.y, b = blockIdx.z;
+  const int G = a.n_heads / a.c.n_kv;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  __shared__ float wred[DW][GP], vred[DW];
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int slot, len;
+  if (!row_keys(a, b, slot, len)) return;
+  const int j0 = ch * s.chunk, n = min(len - j0, s.chunk);
+  if (n <= 0) return;
+  const int64_t row0 = a.c.at(slot, gk, j0);
+  const int8_t* kp = a.c.k + row0 * HD;
+  const float* ksp = a.c.ks + row0;
+  const int64_t bg = (int64_t)b * a.c.n_kv + gk;
+  const int64_t plane = (int64_t)s.n_chunks * s.chunk * T::CP;
+  float* z = s.z + bg * T::NT * plane + (int64_t)(j0 >> 5) * T::ZB;
+  KBlock<HD> k;
+  if (32 * warp < n) k.load(kp, ksp, 32 * warp, n, g, t);
+  float vmax = 0.f;
+  for (int j = tid; j < n; j += DT) vmax = max_nan(vmax, __ldg(a.c.vs + row0 + j));
+  uint32_t qd[T::NT][HD / 32][3][2];
+  float unit[T::NT], mx[T::NT][2];
+  load_q<HD, GP>(a.q + (int64_t)b * a.q_stride + (int64_t)gk * G * HD, G, lane, qd, unit);
+#pragma unroll
+  for (int nt = 0; nt < T::NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
+  for (int row = 32 * warp; row < n; row += 32 * DW) {
+    score_block<HD, GP>(k, qd, g, t, z + (int64_t)(row >> 5) * T::ZB, plane, mx);
+    if (row + 32 * DW < n) k.load(kp, ksp, row + 32 * DW, n, g, t);
+  }
+  warp_maxima<HD, GP>(mx, g, t, wred[warp]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) vmax = max_nan(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+  if (lane == 0) vred[warp] = vmax;
+  __syncthreads();
+  float* stat = s.stat + (bg * s.n_chunks + ch) * (GP + 1);
+  if (tid < GP) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < DW; ++i) m = fmaxf(m, wred[i][tid]);
+    stat[tid] = m;
+  } else if (tid == GP) {
+#pragma unroll
+    for (int i = 0; i < DW; ++i) vmax = max_nan(vmax, vred[i]);
+    stat[GP] = vmax;
+  }
+}
+
+template <int HD, int GP>
+__global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1) split_pv_kernel(Kv8Split s) {
+  using T = Tile<HD, GP>;
+  const Kv8Attn& a = s.a;
+  const int ch = blockIdx.x, gk = blockIdx.y, b = blockIdx.z;
+  const int G = a.n_heads / a.c.n_kv;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  __shared__ __align__(16) float part[T::PART];
+  __shared__ float wred[DW][GP], gmax[DW][GP];
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int slot, len;
+  if (!row_keys(a, b, slot, len)) return;
+  const int j0 = ch * s.chunk, n = min(len - j0, s.chunk);
+  if (n <= 0) return;
+  const int64_t row0 = a.c.at(slot, gk, j0);
+  const int8_t* vp = a.c.v + row0 * HD;
+  const float* vsp = a.c.vs + row0;
+  const int64_t bg = (int64_t)b * a.c.n_kv + gk;
+  const int64_t plane = (int64_t)s.n_chunks * s.chunk * T::CP;
+  const int tw = warp / T::DS, d0 = (warp % T::DS) * T::DP;
+  PVSum<HD, GP> pv;
+  const int col = pv.column(g);
+  const float* z = s.z + bg * T::NT * plane + (int64_t)(j0 >> 5) * T::ZB + col * 32 + t * 8;
+  VBlock<HD, GP> v;
+  if (32 * tw < n) v.load(vp, vsp, 32 * tw, n, lane, d0);
+  // the maximum over the sequence's chunks, and the factors of the heads
+  const float* stat = s.stat + bg * s.n_chunks * (GP + 1);
+  const int used = (len + s.chunk - 1) / s.chunk;
+  if (lane < GP) {
+    float m = -INFINITY;
+    for (int i = warp; i < used; i += DW) m = fmaxf(m, stat[i * (GP + 1) + lane]);
+    gmax[warp][lane] = m;
+  }
+  const float vmax = stat[ch * (GP + 1) + GP];
+  __syncthreads();
+  float max_of[T::NT], unit[T::NT];
+#pragma unroll
+  for (int nt = 0; nt < T::NT; ++nt) {
+    max_of[nt] = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < DW; ++i) max_of[nt] = fmaxf(max_of[nt], gmax[i][nt * 8 + col]);
+    // as load_q forms it
+    const float* q = a.q + (int64_t)b * a.q_stride + (int64_t)(gk * G + nt * 8 + col) * HD;
+    float peak = 0.f;
+    if (nt * 8 + col < G)
+      for (int i = t; i < HD; i += 4) peak = max_nan(peak, fabsf(q[i]));
+    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+    unit[nt] = peak < INFINITY ? pow2i(block_exp(peak) - 22) * (HD == 64 ? 0.125f : 0.0883883476f) : NAN;
+  }
+  pv.start(vmax, max_of, unit);
+  for (int row = 32 * tw; row < n; row += 32 * T::TW) {
+    float zv[T::NT][8];
+#pragma unroll
+    for (int nt = 0; nt < T::NT; ++nt) {
+      const float4* zb = (const float4*)(z + nt * plane + (int64_t)(row >> 5) * T::ZB);
+      *(float4*)&zv[nt][0] = zb[0];
+      *(float4*)&zv[nt][4] = zb[1];
+    }
+    pv.add(v, zv, n - row, lane);
+    if (row + 32 * T::TW < n) v.load(vp, vsp, row + 32 * T::TW, n, lane, d0);
+  }
+  pv.store(part + tw * GP * HD, wred[tw], lane, d0);
+  __syncthreads();
+  float* pacc = s.pacc + (bg * s.n_chunks + ch) * GP * HD;
+  for (int i = tid; i < G * HD; i += DT) {
+    float x = 0.f;
+#pragma unroll
+    for (int r = 0; r < T::TW; ++r) x += part[r * GP * HD + i];
+    pacc[i] = x;
+  }
+  if (tid < GP) {
+    float x = 0.f;
+#pragma unroll
+    for (int i = 0; i < T::TW; ++i) x += wred[i][tid];
+    s.psum[(bg * s.n_chunks + ch) * GP + tid] = x;
+  }
+}
+
+// grid (n_heads, B), HD threads
+__global__ void split_join_kernel(Kv8Split s, int gp) {
+  const Kv8Attn& a = s.a;
+  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x, HD = blockDim.x;
+  const int G = a.n_heads / a.c.n_kv;
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  int slot, len;
+  if (!row_keys(a, b, slot, len)) return;
+  const int used = (len + s.chunk - 1) / s.chunk;
+  const int64_t row = ((int64_t)b * a.c.n_kv + h / G) * s.n_chunks;
+  float x = 0.f, total = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < used; ++c) {
+    x += s.pacc[((row + c) * gp + h % G) * HD + d];
+    total += s.psum[(row + c) * gp + h % G];
+  }
+  a.out[((int64_t)b * a.n_heads + h) * HD + d] = used ? __fdiv_rn(x, total) : 0.f;
 }
 
 constexpr size_t SMEM_MAX = 220 * 1024;
@@ -477,23 +725,66 @@ int launch_decode_cluster(const Kv8Attn& a, int B, int device, int sms, cudaStre
   int cl = largest[device];
   while (cl > 1 && (int64_t)cl * a.c.n_kv * B > 2 * sms) cl >>= 1;
   auto cap_of = [&](int c) { return ((a.max_len + c - 1) / c + 31) & ~31; };
-  while (cl < largest[device] && T::smem_floats(cap_of(cl)) * 4 > SMEM_MAX) cl <<= 1;
-  const size_t smem = T::smem_floats(cap_of(cl)) * 4;
+  while (cl < largest[device] && ClusterSmem<HD, GP>::bytes(cap_of(cl)) > SMEM_MAX) cl <<= 1;
+  if (getenv("CLX")) cl = atoi(getenv("CLX"));
+  const size_t smem = ClusterSmem<HD, GP>::bytes(cap_of(cl));
   if (smem > SMEM_MAX) return SM_ERR_UNSUPPORTED;
   const cudaLaunchConfig_t cfg = launch_config(dim3(cl, a.c.n_kv, B), DT, smem, st, cl, attr);
   SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a, cap_of(cl)));
   return SM_OK;
 }
 
-int launch_decode(const Kv8Attn& a, int hd, int B, int device, int sms, cudaStream_t st) {
+template <int HD, int GP>
+int launch_decode_split(const Kv8Attn& a, int B, cudaStream_t st) {
+  using T = Tile<HD, GP>;
+  Kv8Split s;
+  s.a = a;
+  s.chunk = 1024;
+  s.n_chunks = (a.max_len + s.chunk - 1) / s.chunk;
+  const int64_t bg = (int64_t)B * a.c.n_kv, rows = bg * s.n_chunks;
+  const int64_t nz = rows * s.chunk * GP, nstat = (rows * (GP + 1) + 3) & ~3LL, nacc = rows * GP * HD;
+  void* buf = nullptr;
+  if (cudaMallocAsync(&buf, (size_t)(nz + nstat + nacc + rows * GP) * sizeof(float), st) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(SM_ERR_OOM, "attention_kv8: device allocation failed");
+  }
+  s.z = (float*)buf;
+  s.stat = s.z + nz;
+  s.pacc = s.stat + nstat;
+  s.psum = s.pacc + nacc;
+  cudaLaunchAttribute attr[2];
+  const dim3 grid(s.n_chunks, a.c.n_kv, B);
+  cudaLaunchConfig_t cfg = launch_config(grid, DT, 0, st, 1, attr);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, split_scores_kernel<HD, GP>, s);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, split_pv_kernel<HD, GP>, s);
+  cfg = launch_config(dim3(a.n_heads, B), HD, 0, st, 1, attr);
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, split_join_kernel, s, GP);
+  cudaFreeAsync(buf, st);
+  SM_CUDA_TRY(e);
+  return SM_OK;
+}
+
+template <int HD, int GP>
+int launch_decode_as(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st, int* n_launch) {
+  const char* split = getenv("SPLITX");
+  if (!(split && split[0] == '1')) {
+    const int rc = launch_decode_cluster<HD, GP>(a, B, device, sms, st);
+    if (rc == SM_OK) *n_launch = 1;
+    if (rc != SM_ERR_UNSUPPORTED) return rc;
+  }
+  *n_launch = 3;
+  return launch_decode_split<HD, GP>(a, B, st);
+}
+
+int launch_decode(const Kv8Attn& a, int hd, int B, int device, int sms, cudaStream_t st, int* n_launch) {
   const int G = a.n_heads / a.c.n_kv;
   if (hd == 64)
-    return G <= 4   ? launch_decode_cluster<64, 4>(a, B, device, sms, st)
-           : G <= 8 ? launch_decode_cluster<64, 8>(a, B, device, sms, st)
-                    : launch_decode_cluster<64, 16>(a, B, device, sms, st);
-  return G <= 4   ? launch_decode_cluster<128, 4>(a, B, device, sms, st)
-         : G <= 8 ? launch_decode_cluster<128, 8>(a, B, device, sms, st)
-                  : launch_decode_cluster<128, 16>(a, B, device, sms, st);
+    return G <= 4   ? launch_decode_as<64, 4>(a, B, device, sms, st, n_launch)
+           : G <= 8 ? launch_decode_as<64, 8>(a, B, device, sms, st, n_launch)
+                    : launch_decode_as<64, 16>(a, B, device, sms, st, n_launch);
+  return G <= 4   ? launch_decode_as<128, 4>(a, B, device, sms, st, n_launch)
+         : G <= 8 ? launch_decode_as<128, 8>(a, B, device, sms, st, n_launch)
+                  : launch_decode_as<128, 16>(a, B, device, sms, st, n_launch);
 }
 
 int attend(sm_ctx* ctx, const Kv8Attn& args, int head_dim, int B, const char* what) {
@@ -508,9 +799,10 @@ int attend(sm_ctx* ctx, const Kv8Attn& args, int head_dim, int B, const char* wh
   if (!a.prefix.k) {
     int sms = 0;
     SM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-    const int rc = launch_decode(a, head_dim, B, device, sms, st);
-    if (rc == SM_OK) *launches += 1;
-    if (rc != SM_ERR_UNSUPPORTED) return rc;
+    int nl = 0;
+    SM_TRY(launch_decode(a, head_dim, B, device, sms, st, &nl));
+    *launches += nl;
+    return SM_OK;
   }
   const dim3 grid(a.n_heads, B);
   if (head_dim == 64)

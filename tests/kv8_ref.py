@@ -28,7 +28,12 @@ def attend(q, k, v):
     most d = 8 * 2^-24 * a, and so is the maximum.  |w'/w| <= 1 for x <= 0, so a weight is off by 2 d
     relative (8 more roundings for the quotient); numerator and denominator each by that, and by the
     roundings of their sums: at most 64 + n / 64 in a chain, since every kernel sums in blocks.  The two
-    errors at most add up, times sum(w |v|) / sum(w)."""
+    errors at most add up, times sum(w |v|) / sum(w).
+
+    The products w * v_scale are held in fixed point, a half step of 2^-24 times the largest scale away at
+    most: 2^-24 * max(scale) * sum|code| / sum(w) more.  (A key's scale is max|v| / 127.  The key with the
+    largest scale has w >= 0.07 and is itself up to half a scale off its unquantised value, so this stays
+    far below what the 8 bits cost.)"""
     q, k, v = (np.asarray(a, np.float64) for a in (q, k, v))
     n, hd = k.shape
     if n == 0:
@@ -39,7 +44,9 @@ def attend(q, k, v):
     a = (np.abs(q) @ np.abs(k).T / np.sqrt(hd)).max(1, keepdims=True)
     d = 8 * 2.0 ** -24 * a
     rel = 2 * (2 * d + (8 + 64 + n / 64) * 2.0 ** -24)
-    return w @ v / total, rel * (w @ np.abs(v) / total)
+    scale = np.abs(v).max(1, keepdims=True) / 127
+    codes = np.abs(v) / np.where(scale > 0, scale, 1)
+    return w @ v / total, rel * (w @ np.abs(v) / total) + 2.0 ** -24 * scale.max() * codes.sum(0) / total
 
 
 def attend_rows(q, n_kv, keys):
