@@ -11,6 +11,7 @@
 
 #include "kv8.cuh"
 #include "kv8_mma.cuh"
+#include "mbar.cuh"
 
 namespace sm {
 namespace {
@@ -25,6 +26,7 @@ struct Kv8Attn {
   int max_len, n_heads;
   float* out;
   int* status;
+  bool q_vec;  // rows of q on 16-byte boundaries
 };
 
 constexpr int THREADS = 128;
@@ -129,7 +131,7 @@ __device__ __forceinline__ int zpos(int head, int g) { return head * 32 + (g & 3
 // q of one kv head's group as digits in B-fragment order; `unit` gets 2^(e - 22) / sqrt(HD) of this
 // lane's column head (lane / 4), the factor of its digit sums (NaN where q is not finite).
 template <int HD, int GP>
-__device__ __forceinline__ void load_q(const float* q, int G, int lane, uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
+__device__ __forceinline__ void load_q(const float* q, bool vec, int G, int lane, uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
                                        float (&unit)[Tile<HD, GP>::NT]) {
   using T = Tile<HD, GP>;
   const int g = lane >> 2, t = lane & 3;
@@ -138,8 +140,14 @@ __device__ __forceinline__ void load_q(const float* q, int G, int lane, uint32_t
     const int h = nt * 8 + g;
     float x[HD / 4];
     float peak = 0.f;
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < HD / 4; ++i) x[i] = h < G ? q[h * HD + (i / 16) * 64 + 16 * t + i % 16] : 0.f;
+      for (int i = 0; i < HD / 4; i += 4)
+        *(float4*)(x + i) = h < G ? __ldg((const float4*)(q + h * HD + (i / 16) * 64 + 16 * t + i % 16)) : float4{};
+    } else {
+#pragma unroll
+      for (int i = 0; i < HD / 4; ++i) x[i] = h < G ? __ldg(q + h * HD + (i / 16) * 64 + 16 * t + i % 16) : 0.f;
+    }
 #pragma unroll
     for (int i = 0; i < HD / 4; ++i) peak = max_nan(peak, fabsf(x[i]));
     peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
@@ -437,7 +445,7 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   for (int j = tid; j < n; j += DT) vmax = max_nan(vmax, __ldg(vsp + j));
   uint32_t qd[T::NT][HD / 32][3][2];
   float unit[T::NT], mx[T::NT][2];
-  load_q<HD, GP>(a.q + (int64_t)b * a.q_stride + (int64_t)gk * G * HD, G, lane, qd, unit);
+  load_q<HD, GP>(a.q + (int64_t)b * a.q_stride + (int64_t)gk * G * HD, a.q_vec, G, lane, qd, unit);
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
   for (int row = 32 * warp; row < n; row += 32 * DW) {
@@ -518,60 +526,139 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   cluster.sync();  // no CTA's shared memory goes before the others have read it
 }
 
-// ---------------------------------------------------------------- decode, long: scores, P V and join as three launches
+// ---------------------------------------------------------------- decode, long: scores, then P V, as two launches
 //
 // Flat grids over chunks of keys, so that nothing waits inside a kernel: the scores of a chunk go to
 // global memory with the chunk's maxima (and its largest V scale), the second kernel reads them back
-// against the maximum over the chunks, the third joins the chunks' sums.  The scores add GP * 8 bytes
-// to the 2 * HD + 8 of a key and mostly stay in L2.  Bound by HBM.
+// against the maximum over the chunks; the CTA that finishes a (sequence, kv head) joins its chunks'
+// sums, in order.  The scores add GP * 8 bytes to the 2 * HD + 8 of a key and mostly stay in L2.  Each warp streams its blocks through a ring of its
+// own (asynchronous copies, no barrier but the warp's), two or more blocks ahead of the one it works on.
+// Bound by HBM.
 struct Kv8Split {
   Kv8Attn a;
   int chunk, n_chunks;  // keys of a chunk (whole blocks); chunks that max_len makes
   float* z;             // [B][n_kv][NT][blocks] score blocks
-  float* stat;          // [B][n_kv][n_chunks][GP + 1] maxima, largest V scale
+  float* stat;          // [B][n_kv][n_chunks][2 * GP + 1] maxima, largest V scale; then the weights' sums
+  int* arrived;         // [B][n_kv] chunks whose P V is done
   float* pacc;          // [B][n_kv][n_chunks][GP][HD]
-  float* psum;          // [B][n_kv][n_chunks][GP]
+};
+
+// 16-byte chunk c of row r of a block sits at c ^ swizzle(r): with it neither the K side (lanes of two
+// rows and 64 bytes at once) nor the V side (four rows, 32 bytes) meets a bank twice.
+template <int HD>
+__device__ __forceinline__ int swizzle(int r) {
+  return HD == 128 ? ((r & 1) << 2) | (r & 2) : r & 2;
+}
+
+// A warp's ring slot: codes of 32 rows, their V scales, then the K scales (scores) or the scores (P V).
+template <int HD, int GP, bool PV>
+struct Slot {
+  using T = Tile<HD, GP>;
+  static constexpr int CODES = 32 * HD;
+  static constexpr int MORE = CODES + 128;
+  static constexpr int BYTES = MORE + (PV ? T::NT * T::ZB * 4 : 128);
+  static constexpr int CTAS = PV ? ((GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1) : (GP == 16 ? 1 : 2);
+  // as many slots as the CTAs of an SM have room for, 3 at least
+  static constexpr int FIT = (CTAS == 2 ? 112 : 220) * 1024 / (DW * BYTES);
+  static constexpr int N = FIT > 6 ? 6 : FIT;
+  static constexpr int RING = DW * N * BYTES;
+  static_assert(N >= 3 && RING >= T::PART * 4, "ring too small");
+
+  // rows at or past n repeat row n - 1; ks only where the scores are formed
+  static __device__ __forceinline__ void fetch(uint32_t to, const int8_t* codes, const float* ks, const float* vs,
+                                               int row, int n, int lane) {
+    constexpr int C = HD / 16, R = 32 / C;  // chunks of a row; rows of 32 chunks
+    const int r = lane / C;
+    const uint32_t dst = to + r * HD + (((lane % C) ^ swizzle<HD>(r)) << 4);
+    const int8_t* src = codes + (int64_t)(row + r) * HD + (lane % C) * 16;
+    if (row + 32 <= n) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) cp16(dst + j * 512, src + j * 512);
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j) cp16(dst + j * 512, src + min(j * R, n - 1 - row - r) * HD);
+    }
+    const int s = min(row + lane, n - 1);
+    cp4(to + CODES + 4 * lane, vs + s);
+    if (!PV) cp4(to + MORE + 4 * lane, ks + s);
+  }
+  // the block's scores, planes `plane` floats apart
+  static __device__ __forceinline__ void fetch_scores(uint32_t to, const float* z, int64_t plane, int row, int lane) {
+#pragma unroll
+    for (int nt = 0; nt < T::NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < T::ZB / 128; ++j)
+        cp16(to + MORE + (nt * T::ZB + j * 128 + lane * 4) * 4,
+             z + nt * plane + (int64_t)(row >> 5) * T::ZB + j * 128 + lane * 4);
+  }
 };
 
 template <int HD, int GP>
-__global__ void __launch_bounds__(DT, GP == 16 ? 1 : 2) split_scores_kernel(Kv8Split s) {
+__global__ void __launch_bounds__(DT, (Slot<HD, GP, false>::CTAS)) split_scores_kernel(Kv8Split s) {
   using T = Tile<HD, GP>;
+  using S = Slot<HD, GP, false>;
   const Kv8Attn& a = s.a;
   const int ch = blockIdx.x, gk = blockIdx.y, b = blockIdx.z;
   const int G = a.n_heads / a.c.n_kv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float wred[DW][GP], vred[DW];
-  asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  // only now: what the next kernel reads before its own wait has then been written
+  asm volatile("griddepcontrol.launch_dependents;");
   int slot, len;
   if (!row_keys(a, b, slot, len)) return;
   const int j0 = ch * s.chunk, n = min(len - j0, s.chunk);
+  if (ch == 0 && tid == 0) s.arrived[(int64_t)b * a.c.n_kv + gk] = 0;
   if (n <= 0) return;
   const int64_t row0 = a.c.at(slot, gk, j0);
   const int8_t* kp = a.c.k + row0 * HD;
   const float* ksp = a.c.ks + row0;
+  const float* vsp = a.c.vs + row0;
   const int64_t bg = (int64_t)b * a.c.n_kv + gk;
   const int64_t plane = (int64_t)s.n_chunks * s.chunk * T::CP;
   float* z = s.z + bg * T::NT * plane + (int64_t)(j0 >> 5) * T::ZB;
-  KBlock<HD> k;
-  if (32 * warp < n) k.load(kp, ksp, 32 * warp, n, g, t);
+  const uint8_t* ring = smem + warp * S::N * S::BYTES;
+  const uint32_t ring_at = smem_u32(ring);
+  // block i of the warp starts at row 32 (warp + DW i), slot i % N
+  auto fetch = [&](int row, int at) {
+    if (row < n) S::fetch(ring_at + at * S::BYTES, kp, ksp, vsp, row, n, lane);
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < S::N - 1; ++i) fetch(32 * (warp + DW * i), i);
   float vmax = 0.f;
-  for (int j = tid; j < n; j += DT) vmax = max_nan(vmax, __ldg(a.c.vs + row0 + j));
   uint32_t qd[T::NT][HD / 32][3][2];
   float unit[T::NT], mx[T::NT][2];
-  load_q<HD, GP>(a.q + (int64_t)b * a.q_stride + (int64_t)gk * G * HD, G, lane, qd, unit);
+  load_q<HD, GP>(a.q + (int64_t)b * a.q_stride + (int64_t)gk * G * HD, a.q_vec, G, lane, qd, unit);
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
+  int at = 0;
   for (int row = 32 * warp; row < n; row += 32 * DW) {
+    cp_wait<S::N - 2>();
+    const uint8_t* p = ring + at * S::BYTES;
+    KBlock<HD> k;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int r = krow(g) + 4 * c;
+#pragma unroll
+      for (int l = 0; l < HD / 64; ++l)
+        *(uint4*)k.w[c][l] = *(const uint4*)(p + r * HD + (((l * 4 + t) ^ swizzle<HD>(g)) << 4));
+      k.s[c] = *(const float*)(p + S::MORE + 4 * r);
+    }
+    vmax = max_nan(vmax, *(const float*)(p + S::CODES + 4 * lane));
+    // the slot of the block before this one is free
+    fetch(row + 32 * DW * (S::N - 1), at == 0 ? S::N - 1 : at - 1);
+    at = at == S::N - 1 ? 0 : at + 1;
     score_block<HD, GP>(k, qd, g, t, z + (int64_t)(row >> 5) * T::ZB, plane, mx);
-    if (row + 32 * DW < n) k.load(kp, ksp, row + 32 * DW, n, g, t);
   }
+  cp_wait<0>();
   warp_maxima<HD, GP>(mx, g, t, wred[warp]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) vmax = max_nan(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
   if (lane == 0) vred[warp] = vmax;
   __syncthreads();
-  float* stat = s.stat + (bg * s.n_chunks + ch) * (GP + 1);
+  float* stat = s.stat + (bg * s.n_chunks + ch) * (2 * GP + 1);
   if (tid < GP) {
     float m = -INFINITY;
 #pragma unroll
@@ -585,68 +672,114 @@ __global__ void __launch_bounds__(DT, GP == 16 ? 1 : 2) split_scores_kernel(Kv8S
 }
 
 template <int HD, int GP>
-__global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1) split_pv_kernel(Kv8Split s) {
+__global__ void __launch_bounds__(DT, (Slot<HD, GP, true>::CTAS)) split_pv_kernel(Kv8Split s) {
   using T = Tile<HD, GP>;
+  using S = Slot<HD, GP, true>;
   const Kv8Attn& a = s.a;
   const int ch = blockIdx.x, gk = blockIdx.y, b = blockIdx.z;
   const int G = a.n_heads / a.c.n_kv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  __shared__ __align__(16) float part[T::PART];
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float wred[DW][GP], gmax[DW][GP];
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  __shared__ bool last;
+  // everything but the scores and maxima was there before the first kernel let this one start
   int slot, len;
   if (!row_keys(a, b, slot, len)) return;
   const int j0 = ch * s.chunk, n = min(len - j0, s.chunk);
-  if (n <= 0) return;
+  if (n <= 0) {
+    if (len == 0 && ch == 0)
+      for (int i = tid; i < G * HD; i += DT) a.out[((int64_t)b * a.n_heads + gk * G) * HD + i] = 0.f;
+    return;
+  }
   const int64_t row0 = a.c.at(slot, gk, j0);
   const int8_t* vp = a.c.v + row0 * HD;
   const float* vsp = a.c.vs + row0;
   const int64_t bg = (int64_t)b * a.c.n_kv + gk;
   const int64_t plane = (int64_t)s.n_chunks * s.chunk * T::CP;
   const int tw = warp / T::DS, d0 = (warp % T::DS) * T::DP;
+  const float* z = s.z + bg * T::NT * plane + (int64_t)(j0 >> 5) * T::ZB;
+  const uint8_t* ring = smem + warp * S::N * S::BYTES;
+  const uint32_t ring_at = smem_u32(ring);
+#pragma unroll
+  for (int i = 0; i < S::N - 1; ++i)
+    if (32 * (tw + T::TW * i) < n)
+      S::fetch(ring_at + i * S::BYTES, vp, nullptr, vsp, 32 * (tw + T::TW * i), n, lane);
+  // the maximum over the sequence's chunks, and the factors of the heads
   PVSum<HD, GP> pv;
   const int col = pv.column(g);
-  const float* z = s.z + bg * T::NT * plane + (int64_t)(j0 >> 5) * T::ZB + col * 32 + t * 8;
-  VBlock<HD, GP> v;
-  if (32 * tw < n) v.load(vp, vsp, 32 * tw, n, lane, d0);
-  // the maximum over the sequence's chunks, and the factors of the heads
-  const float* stat = s.stat + bg * s.n_chunks * (GP + 1);
+  float* stat = s.stat + bg * s.n_chunks * (2 * GP + 1);
   const int used = (len + s.chunk - 1) / s.chunk;
+  float max_of[T::NT], unit[T::NT];
+#pragma unroll
+  for (int nt = 0; nt < T::NT; ++nt) {
+    // as load_q forms it
+    const float* q = a.q + (int64_t)b * a.q_stride + (int64_t)(gk * G + nt * 8 + col) * HD;
+    float peak = 0.f;
+    if (nt * 8 + col < G) {
+#pragma unroll 8
+      for (int i = t; i < HD; i += 4) peak = max_nan(peak, fabsf(q[i]));
+    }
+    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+    unit[nt] = peak < INFINITY ? pow2i(block_exp(peak) - 22) * (HD == 64 ? 0.125f : 0.0883883476f) : NAN;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+#pragma unroll
+  for (int i = 0; i < S::N - 1; ++i) {
+    const int row = 32 * (tw + T::TW * i);
+    if (row < n) S::fetch_scores(ring_at + i * S::BYTES, z, plane, row, lane);
+    cp_commit();  // the first group holds all of the codes so far
+  }
   if (lane < GP) {
     float m = -INFINITY;
-    for (int i = warp; i < used; i += DW) m = fmaxf(m, stat[i * (GP + 1) + lane]);
+    for (int i = warp; i < used; i += DW) m = fmaxf(m, stat[i * (2 * GP + 1) + lane]);
     gmax[warp][lane] = m;
   }
-  const float vmax = stat[ch * (GP + 1) + GP];
+  const float vmax = stat[ch * (2 * GP + 1) + GP];
   __syncthreads();
-  float max_of[T::NT], unit[T::NT];
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) {
     max_of[nt] = -INFINITY;
 #pragma unroll
     for (int i = 0; i < DW; ++i) max_of[nt] = fmaxf(max_of[nt], gmax[i][nt * 8 + col]);
-    // as load_q forms it
-    const float* q = a.q + (int64_t)b * a.q_stride + (int64_t)(gk * G + nt * 8 + col) * HD;
-    float peak = 0.f;
-    if (nt * 8 + col < G)
-      for (int i = t; i < HD; i += 4) peak = max_nan(peak, fabsf(q[i]));
-    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-    unit[nt] = peak < INFINITY ? pow2i(block_exp(peak) - 22) * (HD == 64 ? 0.125f : 0.0883883476f) : NAN;
   }
   pv.start(vmax, max_of, unit);
+  int at = 0;
   for (int row = 32 * tw; row < n; row += 32 * T::TW) {
+    cp_wait<S::N - 2>();
+    const uint8_t* p = ring + at * S::BYTES;
     float zv[T::NT][8];
 #pragma unroll
     for (int nt = 0; nt < T::NT; ++nt) {
-      const float4* zb = (const float4*)(z + nt * plane + (int64_t)(row >> 5) * T::ZB);
+      const float4* zb = (const float4*)(p + S::MORE) + (nt * T::ZB + col * 32 + t * 8) / 4;
       *(float4*)&zv[nt][0] = zb[0];
       *(float4*)&zv[nt][4] = zb[1];
     }
+    VBlock<HD, GP> v;
+    v.s = row + lane < n ? *(const float*)(p + S::CODES + 4 * lane) : 0.f;
+    const int byte = d0 + g * T::VB;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint8_t* r = p + (t + 4 * i) * HD + (((byte >> 4) ^ swizzle<HD>(t)) << 4) + (byte & 15);
+      if constexpr (T::VB == 16)
+        *(uint4*)v.w[i] = *(const uint4*)r;
+      else
+        *(uint2*)v.w[i] = *(const uint2*)r;
+    }
+    const int next = row + 32 * T::TW * (S::N - 1);
+    if (next < n) {
+      const uint32_t to = ring_at + (at == 0 ? S::N - 1 : at - 1) * S::BYTES;
+      S::fetch(to, vp, nullptr, vsp, next, n, lane);
+      S::fetch_scores(to, z, plane, next, lane);
+    }
+    cp_commit();
+    at = at == S::N - 1 ? 0 : at + 1;
     pv.add(v, zv, n - row, lane);
-    if (row + 32 * T::TW < n) v.load(vp, vsp, row + 32 * T::TW, n, lane, d0);
   }
+  cp_wait<0>();
+  __syncthreads();  // the rings are done
+  float* part = (float*)smem;  // [TW][GP][HD]
   pv.store(part + tw * GP * HD, wred[tw], lane, d0);
   __syncthreads();
   float* pacc = s.pacc + (bg * s.n_chunks + ch) * GP * HD;
@@ -660,28 +793,24 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
     float x = 0.f;
 #pragma unroll
     for (int i = 0; i < T::TW; ++i) x += wred[i][tid];
-    s.psum[(bg * s.n_chunks + ch) * GP + tid] = x;
+    stat[ch * (2 * GP + 1) + GP + 1 + tid] = x;
   }
-}
-
-// grid (n_heads, B), HD threads
-__global__ void split_join_kernel(Kv8Split s, int gp) {
-  const Kv8Attn& a = s.a;
-  const int h = blockIdx.x, b = blockIdx.y, d = threadIdx.x, HD = blockDim.x;
-  const int G = a.n_heads / a.c.n_kv;
-  asm volatile("griddepcontrol.launch_dependents;");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  int slot, len;
-  if (!row_keys(a, b, slot, len)) return;
-  const int used = (len + s.chunk - 1) / s.chunk;
-  const int64_t row = ((int64_t)b * a.c.n_kv + h / G) * s.n_chunks;
-  float x = 0.f, total = 0.f;
-#pragma unroll 4
-  for (int c = 0; c < used; ++c) {
-    x += s.pacc[((row + c) * gp + h % G) * HD + d];
-    total += s.psum[(row + c) * gp + h % G];
+  // the last CTA of this (sequence, kv head) joins the chunks, always in their order
+  __threadfence();
+  __syncthreads();
+  if (tid == 0) last = atomicAdd(s.arrived + bg, 1) == used - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  for (int i = tid; i < G * HD; i += DT) {
+    float x = 0.f, total = 0.f;
+#pragma unroll 8
+    for (int c = 0; c < used; ++c) {
+      x += __ldcg(s.pacc + (bg * s.n_chunks + c) * GP * HD + i);
+      total += __ldcg(stat + c * (2 * GP + 1) + GP + 1 + i / HD);
+    }
+    a.out[((int64_t)b * a.n_heads + gk * G) * HD + i] = __fdiv_rn(x, total);
   }
-  a.out[((int64_t)b * a.n_heads + h) * HD + d] = used ? __fdiv_rn(x, total) : 0.f;
 }
 
 constexpr size_t SMEM_MAX = 220 * 1024;
@@ -735,30 +864,43 @@ int launch_decode_cluster(const Kv8Attn& a, int B, int device, int sms, cudaStre
 }
 
 template <int HD, int GP>
-int launch_decode_split(const Kv8Attn& a, int B, cudaStream_t st) {
-  using T = Tile<HD, GP>;
+int launch_decode_split(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st) {
+  auto scores = split_scores_kernel<HD, GP>;
+  auto pv = split_pv_kernel<HD, GP>;
+  using SK = Slot<HD, GP, false>;
+  using SV = Slot<HD, GP, true>;
+  static bool ready[64] = {};
+  if (device >= 64) return fail(SM_ERR_UNSUPPORTED, "attention_kv8: device id too large");
+  if (!ready[device]) {
+    SM_CUDA_TRY(cudaFuncSetAttribute(scores, cudaFuncAttributeMaxDynamicSharedMemorySize, SK::RING));
+    SM_CUDA_TRY(cudaFuncSetAttribute(pv, cudaFuncAttributeMaxDynamicSharedMemorySize, SV::RING));
+    ready[device] = true;
+  }
   Kv8Split s;
   s.a = a;
-  s.chunk = 1024;
+  const int64_t bg = (int64_t)B * a.c.n_kv;
+  const char* cx = getenv("CHX");
+  // one wave of CTAs where that makes chunks of at most 4096 keys
+  const int waves = (int)max((int64_t)1, (int64_t)SV::CTAS * sms / bg);
+  s.chunk = min(cx ? atoi(cx) : 2048, max(512, ((a.max_len + waves - 1) / waves + 31) & ~31));
   s.n_chunks = (a.max_len + s.chunk - 1) / s.chunk;
-  const int64_t bg = (int64_t)B * a.c.n_kv, rows = bg * s.n_chunks;
-  const int64_t nz = rows * s.chunk * GP, nstat = (rows * (GP + 1) + 3) & ~3LL, nacc = rows * GP * HD;
+  const int64_t rows = bg * s.n_chunks;
+  const int64_t nz = rows * s.chunk * GP, nstat = rows * (2 * GP + 1), nacc = rows * GP * HD;
   void* buf = nullptr;
-  if (cudaMallocAsync(&buf, (size_t)(nz + nstat + nacc + rows * GP) * sizeof(float), st) != cudaSuccess) {
+  if (cudaMallocAsync(&buf, (size_t)(nz + nacc + nstat + bg) * sizeof(float), st) != cudaSuccess) {
     cudaGetLastError();
     return fail(SM_ERR_OOM, "attention_kv8: device allocation failed");
   }
   s.z = (float*)buf;
-  s.stat = s.z + nz;
-  s.pacc = s.stat + nstat;
-  s.psum = s.pacc + nacc;
+  s.pacc = s.z + nz;
+  s.stat = s.pacc + nacc;
+  s.arrived = (int*)(s.stat + nstat);
   cudaLaunchAttribute attr[2];
   const dim3 grid(s.n_chunks, a.c.n_kv, B);
-  cudaLaunchConfig_t cfg = launch_config(grid, DT, 0, st, 1, attr);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, split_scores_kernel<HD, GP>, s);
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, split_pv_kernel<HD, GP>, s);
-  cfg = launch_config(dim3(a.n_heads, B), HD, 0, st, 1, attr);
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, split_join_kernel, s, GP);
+  cudaLaunchConfig_t cfg = launch_config(grid, DT, SK::RING, st, 1, attr);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, scores, s);
+  cfg.dynamicSmemBytes = SV::RING;
+  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, pv, s);
   cudaFreeAsync(buf, st);
   SM_CUDA_TRY(e);
   return SM_OK;
@@ -772,8 +914,8 @@ int launch_decode_as(const Kv8Attn& a, int B, int device, int sms, cudaStream_t 
     if (rc == SM_OK) *n_launch = 1;
     if (rc != SM_ERR_UNSUPPORTED) return rc;
   }
-  *n_launch = 3;
-  return launch_decode_split<HD, GP>(a, B, st);
+  *n_launch = 2;
+  return launch_decode_split<HD, GP>(a, B, device, sms, st);
 }
 
 int launch_decode(const Kv8Attn& a, int hd, int B, int device, int sms, cudaStream_t st, int* n_launch) {
@@ -814,6 +956,8 @@ int attend(sm_ctx* ctx, const Kv8Attn& args, int head_dim, int B, const char* wh
   return SM_OK;
 }
 
+bool q_rows_vec(const float* q, int64_t q_stride) { return (uintptr_t)q % 16 == 0 && q_stride % 4 == 0; }
+
 int check_attn(sm_ctx* ctx, const sm_kv8* c, const float* q, int64_t q_stride, const int* seq_ids, const int* lens,
                int max_len, int B, int n_heads, const float* out, const char* what) {
   const std::string w(what);
@@ -841,7 +985,7 @@ SM_API int sm_attention_decode_kv8(sm_ctx* ctx, const sm_kv8* cache, const float
   const char* what = "attention_decode_kv8";
   SM_TRY(check_attn(ctx, cache, q, q_stride, seq_ids, lens, max_len, B, n_heads, out, what));
   if (B == 0) return SM_OK;
-  Kv8Attn a{kv8_view(cache), {}, 0, 0, q, q_stride, seq_ids, lens, max_len, n_heads, out, nullptr};
+  Kv8Attn a{kv8_view(cache), {}, 0, 0, q, q_stride, seq_ids, lens, max_len, n_heads, out, nullptr, q_rows_vec(q, q_stride)};
   return attend(ctx, a, cache->head_dim, B, what);
 }
 
@@ -860,7 +1004,7 @@ SM_API int sm_attention_shared_kv8(sm_ctx* ctx, const sm_kv8* prefix, int prefix
   SM_TRY(check_attn(ctx, cache, q, q_stride, seq_ids, lens, max_len, B, n_heads, out, what));
   if (B == 0) return SM_OK;
   Kv8Attn a{kv8_view(cache), kv8_view(prefix), prefix_seq, prefix_len, q, q_stride, seq_ids, lens, max_len, n_heads,
-            out, nullptr};
+            out, nullptr, q_rows_vec(q, q_stride)};
   return attend(ctx, a, cache->head_dim, B, what);
 }
 

@@ -88,4 +88,18 @@ __device__ __forceinline__ void ld_codes(const int8_t* p, uint32_t (&w)[2]) {
   asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
 }
 
+// Asynchronous copies into shared memory, in groups that a warp waits for itself
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {  // all but the N newest groups are here, for every lane
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+  __syncwarp();
+}
+
 }  // namespace sm
