@@ -268,12 +268,18 @@ struct VBlock {
 template <int HD, int GP>
 struct PVSum {
   using T = Tile<HD, GP>;
+  // A lane's head is column g of each tile and its keys are t + 4 i, i = 0..7.  With P as A, lanes g and
+  // g + 4 share head g & 3: the first takes i = 0..3, the second i = 4..7.
+  static constexpr int NZ = T::PA ? 4 : 8;
+  static __device__ __forceinline__ int column(int g) { return T::PA ? g & 3 : g; }
+  // where the lane's scores of a block and tile begin
+  static __device__ __forceinline__ int zstart(int g, int t) {
+    return T::PA ? (g & 3) * 32 + t * 8 + (g >> 2) * 4 : g * 32 + t * 8;
+  }
+
   float m[T::NT], unit[T::NT], esum[T::NT];  // of this lane's head: factored maximum, factor, sum of weights
   float mult, back;                          // fixed point: e = 1 at scale vmax is 2^23 - 8
   int acc[T::MD][T::MT][4];
-
-  // A lane's head is column g of each tile; with P as A both halves of the rows hold heads 0..3.
-  static __device__ __forceinline__ int column(int g) { return T::PA ? g & 3 : g; }
 
   // Scales under 1e-30 keep the resolution of 1e-30, so that neither factor overflows.
   __device__ __forceinline__ void start(float vmax, const float (&max_of)[T::NT], const float (&unit_of)[T::NT]) {
@@ -290,32 +296,33 @@ struct PVSum {
         for (int e = 0; e < 4; ++e) acc[i][c][e] = 0;
   }
 
-  // zv: the lane's 8 scores of each tile; keys: how many of the block's 32 exist.  v is used up.
-  __device__ __forceinline__ void add(VBlock<HD, GP>& v, const float (&zv)[T::NT][8], int keys, int lane) {
+  // zv: the lane's scores of each tile; keys: how many of the block's 32 exist.  v is used up.
+  __device__ __forceinline__ void add(VBlock<HD, GP>& v, const float (&zv)[T::NT][NZ], int keys, int lane) {
     const int g = lane >> 2, t = lane & 3;
+    const int first = T::PA ? t + (g >> 2) * 16 : t;
     const float vsm = v.s * mult;
-    uint32_t dg[T::NT][3][2];
+    uint32_t dg[T::NT][3][NZ / 4];
 #pragma unroll
     for (int nt = 0; nt < T::NT; ++nt) {
-      float e[8];
+      float e[NZ];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = kv8_weight(fmaf(zv[nt][i], unit[nt], -m[nt]));
+      for (int i = 0; i < NZ; ++i) e[i] = kv8_weight(fmaf(zv[nt][i], unit[nt], -m[nt]));
       if (keys < 32) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (t + 4 * i >= keys) e[i] = 0.f;
+        for (int i = 0; i < NZ; ++i)
+          if (first + 4 * i >= keys) e[i] = 0.f;
       }
       float part = 0.f;
-      uint32_t p[8];
+      uint32_t p[NZ];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < NZ; ++i) {
         part += e[i];
         // e * scale lies in [0, 2^23): added to 2^23 it is the mantissa, rounded
-        p[i] = __float_as_uint(fmaf(e[i], __shfl_sync(0xffffffffu, vsm, t + 4 * i), 8388608.f));
+        p[i] = __float_as_uint(fmaf(e[i], __shfl_sync(0xffffffffu, vsm, first + 4 * i), 8388608.f));
       }
       esum[nt] += part;
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
+      for (int half = 0; half < NZ / 4; ++half)
         bytes3(p[4 * half], p[4 * half + 1], p[4 * half + 2], p[4 * half + 3], dg[nt][0][half], dg[nt][1][half],
                dg[nt][2][half]);
     }
@@ -325,9 +332,12 @@ struct PVSum {
       transpose4(v.w[4][c], v.w[5][c], v.w[6][c], v.w[7][c]);
     }
     if constexpr (T::PA) {
-      // rows: digit 0 of heads 0..3, digit 1, digit 2, zeros
-      const uint32_t a0 = g < 4 ? dg[0][0][0] : dg[0][1][0], a2 = g < 4 ? dg[0][0][1] : dg[0][1][1];
-      const uint32_t a1 = g < 4 ? dg[0][2][0] : 0u, a3 = g < 4 ? dg[0][2][1] : 0u;
+      // rows: digit 0 of heads 0..3, digit 1, digit 2, zeros; lanes g and g + 4 exchange what the other's rows need
+      const bool low = g < 4;
+      const uint32_t x = __shfl_xor_sync(0xffffffffu, low ? dg[0][1][0] : dg[0][0][0], 16);
+      const uint32_t y = __shfl_xor_sync(0xffffffffu, dg[0][2][0], 16);
+      const uint32_t a0 = low ? dg[0][0][0] : x, a2 = low ? x : dg[0][1][0];
+      const uint32_t a1 = low ? dg[0][2][0] : 0u, a3 = low ? y : 0u;
 #pragma unroll
       for (int c = 0; c < T::MT; ++c)
         mma_u8s8_acc(acc[0][c], a0, a1, a2, a3, v.w[c & 3][c >> 2], v.w[4 + (c & 3)][c >> 2]);
@@ -351,6 +361,7 @@ struct PVSum {
     for (int nt = 0; nt < T::NT; ++nt) {
       esum[nt] += __shfl_xor_sync(0xffffffffu, esum[nt], 1);
       esum[nt] += __shfl_xor_sync(0xffffffffu, esum[nt], 2);
+      if (T::PA) esum[nt] += __shfl_xor_sync(0xffffffffu, esum[nt], 16);
       if (t == 0 && g < T::CP && d0 == 0) sums[nt * 8 + g] = esum[nt];
     }
     if constexpr (T::PA) {
@@ -487,13 +498,12 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   }
   pv.start(vmax, max_of, unit);
   for (int row = 32 * tw; row < n; row += 32 * T::TW) {
-    float zv[T::NT][8];
+    float zv[T::NT][pv.NZ];
 #pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt) {
-      const float4* zb = (const float4*)(z + nt * plane + (row >> 5) * T::ZB + col * 32 + t * 8);
-      *(float4*)&zv[nt][0] = zb[0];
-      *(float4*)&zv[nt][4] = zb[1];
-    }
+    for (int nt = 0; nt < T::NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < pv.NZ; i += 4)
+        *(float4*)&zv[nt][i] = *(const float4*)(z + nt * plane + (row >> 5) * T::ZB + pv.zstart(g, t) + i);
     pv.add(v, zv, n - row, lane);
     if (row + 32 * T::TW < n) v.load(vp, vsp, row + 32 * T::TW, n, lane, d0);
   }
@@ -566,17 +576,17 @@ struct Slot {
 
   // rows at or past n repeat row n - 1; ks only where the scores are formed
   static __device__ __forceinline__ void fetch(uint32_t to, const int8_t* codes, const float* ks, const float* vs,
-                                               int row, int n, int lane) {
+                                               int row, int n, int lane, uint64_t policy) {
     constexpr int C = HD / 16, R = 32 / C;  // chunks of a row; rows of 32 chunks
     const int r = lane / C;
     const uint32_t dst = to + r * HD + (((lane % C) ^ swizzle<HD>(r)) << 4);
     const int8_t* src = codes + (int64_t)(row + r) * HD + (lane % C) * 16;
     if (row + 32 <= n) {
 #pragma unroll
-      for (int j = 0; j < C; ++j) cp16(dst + j * 512, src + j * 512);
+      for (int j = 0; j < C; ++j) cp16_once(dst + j * 512, src + j * 512, policy);
     } else {
 #pragma unroll
-      for (int j = 0; j < C; ++j) cp16(dst + j * 512, src + min(j * R, n - 1 - row - r) * HD);
+      for (int j = 0; j < C; ++j) cp16_once(dst + j * 512, src + min(j * R, n - 1 - row - r) * HD, policy);
     }
     const int s = min(row + lane, n - 1);
     cp4(to + CODES + 4 * lane, vs + s);
@@ -620,9 +630,10 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, false>::CTAS)) split_scores_
   float* z = s.z + bg * T::NT * plane + (int64_t)(j0 >> 5) * T::ZB;
   const uint8_t* ring = smem + warp * S::N * S::BYTES;
   const uint32_t ring_at = smem_u32(ring);
+  const uint64_t policy = l2_evict_first_policy();
   // block i of the warp starts at row 32 (warp + DW i), slot i % N
   auto fetch = [&](int row, int at) {
-    if (row < n) S::fetch(ring_at + at * S::BYTES, kp, ksp, vsp, row, n, lane);
+    if (row < n) S::fetch(ring_at + at * S::BYTES, kp, ksp, vsp, row, n, lane, policy);
     cp_commit();
   };
 #pragma unroll
@@ -700,10 +711,11 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, true>::CTAS)) split_pv_kerne
   const float* z = s.z + bg * T::NT * plane + (int64_t)(j0 >> 5) * T::ZB;
   const uint8_t* ring = smem + warp * S::N * S::BYTES;
   const uint32_t ring_at = smem_u32(ring);
+  const uint64_t policy = l2_evict_first_policy();
 #pragma unroll
   for (int i = 0; i < S::N - 1; ++i)
     if (32 * (tw + T::TW * i) < n)
-      S::fetch(ring_at + i * S::BYTES, vp, nullptr, vsp, 32 * (tw + T::TW * i), n, lane);
+      S::fetch(ring_at + i * S::BYTES, vp, nullptr, vsp, 32 * (tw + T::TW * i), n, lane, policy);
   // the maximum over the sequence's chunks, and the factors of the heads
   PVSum<HD, GP> pv;
   const int col = pv.column(g);
@@ -749,13 +761,12 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, true>::CTAS)) split_pv_kerne
   for (int row = 32 * tw; row < n; row += 32 * T::TW) {
     cp_wait<S::N - 2>();
     const uint8_t* p = ring + at * S::BYTES;
-    float zv[T::NT][8];
+    float zv[T::NT][pv.NZ];
 #pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt) {
-      const float4* zb = (const float4*)(p + S::MORE) + (nt * T::ZB + col * 32 + t * 8) / 4;
-      *(float4*)&zv[nt][0] = zb[0];
-      *(float4*)&zv[nt][4] = zb[1];
-    }
+    for (int nt = 0; nt < T::NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < pv.NZ; i += 4)
+        *(float4*)&zv[nt][i] = *((const float4*)(p + S::MORE) + (nt * T::ZB + pv.zstart(g, t) + i) / 4);
     VBlock<HD, GP> v;
     v.s = row + lane < n ? *(const float*)(p + S::CODES + 4 * lane) : 0.f;
     const int byte = d0 + g * T::VB;
@@ -770,7 +781,7 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, true>::CTAS)) split_pv_kerne
     const int next = row + 32 * T::TW * (S::N - 1);
     if (next < n) {
       const uint32_t to = ring_at + (at == 0 ? S::N - 1 : at - 1) * S::BYTES;
-      S::fetch(to, vp, nullptr, vsp, next, n, lane);
+      S::fetch(to, vp, nullptr, vsp, next, n, lane, policy);
       S::fetch_scores(to, z, plane, next, lane);
     }
     cp_commit();
