@@ -202,9 +202,9 @@ typedef struct sm_kv8 {
 /* Quantise K and V rows into the cache: row i goes to position positions[i] of slot
  * seq_ids[i].  k, v: row i at k + i * row_stride, [n_kv][head_dim] fp32 (row_stride
  * in floats, >= n_kv * head_dim, so rows may sit inside a fused Q|K|V row).
- * Per kv head: scale = max|x| / 127 in fp32, code = x / scale rounded to the
- * nearest integer, ties to even (exactly, whatever the magnitudes); zeros give
- * scale 0 and codes 0.  A head with an infinity or NaN gets scale NaN and codes 0,
+ * Per kv head: scale = max|x| * (1 / 127) in fp32, code = x / scale rounded to the
+ * nearest integer, ties to even (exactly, whatever the magnitudes); a scale of 0
+ * (zeros, or values that all round away) has codes 0.  A head with an infinity or NaN gets scale NaN and codes 0,
  * so it reads back as NaN.  Each (slot, position) at most once per call: what two
  * rows with the same target leave in it is unspecified. */
 SM_API int sm_kv8_write(sm_ctx* ctx, const sm_kv8* cache, const float* k, const float* v, int64_t row_stride,

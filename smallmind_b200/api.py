@@ -343,42 +343,49 @@ class KV8Cache:
 
     def __init__(self, ctx: CudaContext, k_ptr: int, v_ptr: int, k_scale_ptr: int, v_scale_ptr: int, max_seqs: int,
                  max_tokens: int, n_kv_heads: int, head_dim: int):
-        self.ctx = ctx
+        self.ctx, self._lib = ctx, L.lib()
         self.view = L.KV8(k_ptr, v_ptr, k_scale_ptr, v_scale_ptr, max_seqs, max_tokens, n_kv_heads, head_dim)
         self.max_seqs, self.max_tokens, self.n_kv_heads, self.head_dim = max_seqs, max_tokens, n_kv_heads, head_dim
 
     def write_device(self, k_ptr: int, v_ptr: int, seq_ptr: int, pos_ptr: int, n_rows: int,
                      row_stride: int | None = None):
         """Quantise n_rows fp32 K and V rows into positions pos[i] of slots seq[i] (sm_kv8_write)."""
-        L.check(L.lib().sm_kv8_write(self.ctx.handle, self.view, k_ptr, v_ptr,
-                                     self.n_kv_heads * self.head_dim if row_stride is None else row_stride, seq_ptr,
-                                     pos_ptr, n_rows), "sm_kv8_write")
+        if row_stride is None:
+            row_stride = self.n_kv_heads * self.head_dim
+        L.check(self._lib.sm_kv8_write(self.ctx.handle, self.view, k_ptr, v_ptr, row_stride, seq_ptr, pos_ptr,
+                                       n_rows), "sm_kv8_write")
 
     def read_device(self, seq_ptr: int, pos_ptr: int, n_rows: int, k_ptr: int | None, v_ptr: int | None,
                     row_stride: int | None = None):
         """Read positions back as fp32 rows (sm_kv8_read); k_ptr or v_ptr may be None."""
-        L.check(L.lib().sm_kv8_read(self.ctx.handle, self.view, seq_ptr, pos_ptr, n_rows, k_ptr, v_ptr,
-                                    self.n_kv_heads * self.head_dim if row_stride is None else row_stride),
+        if row_stride is None:
+            row_stride = self.n_kv_heads * self.head_dim
+        L.check(self._lib.sm_kv8_read(self.ctx.handle, self.view, seq_ptr, pos_ptr, n_rows, k_ptr, v_ptr, row_stride),
                 "sm_kv8_read")
 
     def attention_decode_device(self, q_ptr: int, seq_ptr: int | None, lens_ptr: int, batch: int, n_heads: int,
                                 out_ptr: int, max_len: int | None = None, q_stride: int | None = None):
         """Decode attention, one query row per sequence (sm_attention_decode_kv8).  max_len: an upper
         bound of this call's lengths (default: the cache's max_tokens)."""
-        L.check(L.lib().sm_attention_decode_kv8(self.ctx.handle, self.view, q_ptr,
-                                                n_heads * self.head_dim if q_stride is None else q_stride, seq_ptr,
-                                                lens_ptr, self.max_tokens if max_len is None else max_len, batch,
-                                                n_heads, out_ptr), "sm_attention_decode_kv8")
+        if q_stride is None:
+            q_stride = n_heads * self.head_dim
+        if max_len is None:
+            max_len = self.max_tokens
+        L.check(self._lib.sm_attention_decode_kv8(self.ctx.handle, self.view, q_ptr, q_stride, seq_ptr, lens_ptr,
+                                                  max_len, batch, n_heads, out_ptr), "sm_attention_decode_kv8")
 
     def attention_shared_device(self, q_ptr: int, prefix: "KV8Cache", prefix_seq: int, prefix_len: int,
                                 seq_ptr: int | None, lens_ptr: int, batch: int, n_heads: int, out_ptr: int,
                                 max_len: int | None = None, q_stride: int | None = None):
         """Decode attention of a batch that shares the first prefix_len positions of one slot of
         ``prefix`` (sm_attention_shared_kv8)."""
-        L.check(L.lib().sm_attention_shared_kv8(self.ctx.handle, prefix.view, prefix_seq, prefix_len, self.view,
-                                                q_ptr, n_heads * self.head_dim if q_stride is None else q_stride,
-                                                seq_ptr, lens_ptr, self.max_tokens if max_len is None else max_len,
-                                                batch, n_heads, out_ptr), "sm_attention_shared_kv8")
+        if q_stride is None:
+            q_stride = n_heads * self.head_dim
+        if max_len is None:
+            max_len = self.max_tokens
+        L.check(self._lib.sm_attention_shared_kv8(self.ctx.handle, prefix.view, prefix_seq, prefix_len, self.view,
+                                                  q_ptr, q_stride, seq_ptr, lens_ptr, max_len, batch, n_heads,
+                                                  out_ptr), "sm_attention_shared_kv8")
 
 
 @dataclass

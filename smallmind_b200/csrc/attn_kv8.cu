@@ -7,7 +7,8 @@
 // partial results against a running maximum cannot be rescaled: the exact maximum comes
 // first and the weights are formed against it.
 #include <cooperative_groups.h>
-#include <cstdlib>
+
+#include <algorithm>
 
 #include "kv8.cuh"
 #include "kv8_mma.cuh"
@@ -95,9 +96,8 @@ __global__ void __launch_bounds__(THREADS) attn_kv8_kernel(Kv8Attn a) {
 // ---------------------------------------------------------------- pieces of the decode kernels
 //
 // Keys are taken in blocks of 32, a warp each:
-//   scores  two 16-key x 8-head MMA tiles.  K codes go from global memory into A fragments as they
-//           lie: a lane takes 16 neighbouring bytes of a row, and q's digits, built once, are in
-//           the matching order.  A lane's four rows are the keys whose scores the P side wants
+//   scores  two 16-key x 8-head MMA tiles.  K codes are A fragments as they lie: a lane takes 16
+//           neighbouring bytes of a row, and q's digits, built once, are in the matching order.  A lane's four rows are the keys whose scores the P side wants
 //           side by side.  Scores are kept without the head's positive factor, which a maximum
 //           does not need;
 //   P V     weights e, and P = e * v_scale in 23-bit fixed point against the largest v_scale of
@@ -169,31 +169,10 @@ __device__ __forceinline__ void load_q(const float* q, bool vec, int G, int lane
 }
 
 // K codes and scales of a block, as a lane holds them: rows krow(g) + 4 c, bytes 16 t .. of each 64.
-// Rows at or past n repeat row n - 1, which leaves a maximum as it is.
 template <int HD>
 struct KBlock {
   uint32_t w[4][HD / 64][4];
   float s[4];
-  __device__ __forceinline__ void load(const int8_t* kp, const float* ksp, int row, int n, int g, int t) {
-    const int r = row + krow(g);
-    const int8_t* p = kp + (int64_t)r * HD + 16 * t;
-    if (row + 32 <= n) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-#pragma unroll
-        for (int l = 0; l < HD / 64; ++l) ld_codes(p + 4 * c * HD + l * 64, w[c][l]);
-        s[c] = __ldg(ksp + r + 4 * c);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int o = min(4 * c, n - 1 - r);
-#pragma unroll
-        for (int l = 0; l < HD / 64; ++l) ld_codes(p + o * HD + l * 64, w[c][l]);
-        s[c] = __ldg(ksp + r + o);
-      }
-    }
-  }
 };
 
 // Scores of a block: to z ([NT] planes `plane` floats apart), and this lane's running maxima of columns 2t, 2t + 1.
@@ -246,22 +225,8 @@ __device__ __forceinline__ void warp_maxima(const float (&mx)[Tile<HD, GP>::NT][
 // V codes of a block: keys t + 4 i, VB dims of each; and the scale of key `lane` (0 past the end).
 template <int HD, int GP>
 struct VBlock {
-  using T = Tile<HD, GP>;
-  uint32_t w[8][T::VB / 4];
+  uint32_t w[8][Tile<HD, GP>::VB / 4];
   float s;
-  __device__ __forceinline__ void load(const int8_t* vp, const float* vsp, int row, int n, int lane, int d0) {
-    const int g = lane >> 2, t = lane & 3;
-    const int8_t* p = vp + (int64_t)(row + t) * HD + d0 + g * T::VB;
-    if (row + 32 <= n) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ld_codes(p + 4 * i * HD, w[i]);
-      s = __ldg(vsp + row + lane);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ld_codes(p + min(4 * i, n - 1 - row - t) * HD, w[i]);
-      s = row + lane < n ? __ldg(vsp + row + lane) : 0.f;
-    }
-  }
 };
 
 // What a warp accumulates of P V, and how P is formed.
@@ -405,30 +370,119 @@ __device__ __forceinline__ bool row_keys(const Kv8Attn& a, int b, int& slot, int
   return true;
 }
 
+// ---------------------------------------------------------------- a warp's ring
+//
+// Each warp streams its blocks through a ring of its own: asynchronous copies, some blocks ahead of the
+// one it works on, and no barrier but the warp's.
+//
+// 16-byte chunk c of row r of a block sits at c ^ swizzle(r): with it neither the K side (lanes of two
+// rows and 64 bytes at once) nor the V side (four rows, 32 bytes) meets a bank twice.
+template <int HD>
+__device__ __forceinline__ int swizzle(int r) {
+  return HD == 128 ? ((r & 1) << 2) | (r & 2) : r & 2;
+}
+
+// One slot: codes of 32 rows, their V scales, then 128 bytes of K scales or (Z) the block's scores.
+template <int HD, int GP, bool Z>
+struct Slot {
+  using T = Tile<HD, GP>;
+  static constexpr int CODES = 32 * HD;
+  static constexpr int MORE = CODES + 128;
+  static constexpr int BYTES = MORE + (Z ? T::NT * T::ZB * 4 : 128);
+
+  // rows at or past n repeat row n - 1; ks nullptr: none
+  static __device__ __forceinline__ void fetch(uint32_t to, const int8_t* codes, const float* ks, const float* vs,
+                                               int row, int n, int lane, uint64_t policy) {
+    constexpr int C = HD / 16, R = 32 / C;  // chunks of a row; rows of 32 chunks
+    const int r = lane / C;
+    const uint32_t dst = to + r * HD + (((lane % C) ^ swizzle<HD>(r)) << 4);
+    const int8_t* src = codes + (int64_t)(row + r) * HD + (lane % C) * 16;
+    if (row + 32 <= n) {
+#pragma unroll
+      for (int j = 0; j < C; ++j) cp16_once(dst + j * 512, src + j * 512, policy);
+    } else {
+#pragma unroll
+      for (int j = 0; j < C; ++j) cp16_once(dst + j * 512, src + min(j * R, n - 1 - row - r) * HD, policy);
+    }
+    const int s = min(row + lane, n - 1);
+    cp4(to + CODES + 4 * lane, vs + s);
+    if (ks) cp4(to + MORE + 4 * lane, ks + s);
+  }
+  // the block's scores, planes `plane` floats apart
+  static __device__ __forceinline__ void fetch_scores(uint32_t to, const float* z, int64_t plane, int row, int lane) {
+#pragma unroll
+    for (int nt = 0; nt < T::NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < T::ZB / 128; ++j)
+        cp16(to + MORE + (nt * T::ZB + j * 128 + lane * 4) * 4,
+             z + nt * plane + (int64_t)(row >> 5) * T::ZB + j * 128 + lane * 4);
+  }
+  static __device__ __forceinline__ void read_k(const uint8_t* p, KBlock<HD>& k, float& vmax, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int r = krow(g) + 4 * c;
+#pragma unroll
+      for (int l = 0; l < HD / 64; ++l)
+        *(uint4*)k.w[c][l] = *(const uint4*)(p + r * HD + (((l * 4 + t) ^ swizzle<HD>(g)) << 4));
+      k.s[c] = *(const float*)(p + MORE + 4 * r);
+    }
+    vmax = max_nan(vmax, *(const float*)(p + CODES + 4 * lane));
+  }
+  // keys: how many of the block's rows exist
+  static __device__ __forceinline__ void read_v(const uint8_t* p, VBlock<HD, GP>& v, int keys, int d0, int lane) {
+    const int g = lane >> 2, t = lane & 3, byte = d0 + g * T::VB;
+    v.s = lane < keys ? *(const float*)(p + CODES + 4 * lane) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint8_t* r = p + (t + 4 * i) * HD + (((byte >> 4) ^ swizzle<HD>(t)) << 4) + (byte & 15);
+      if constexpr (T::VB == 16)
+        *(uint4*)v.w[i] = *(const uint4*)r;
+      else
+        *(uint2*)v.w[i] = *(const uint2*)r;
+    }
+  }
+};
+
+// Largest of a warp's values, NaN if any is
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
 // ---------------------------------------------------------------- decode, short: one cluster per (sequence, kv head)
 //
 // One launch: the keys are split over the cluster's CTAs, the scores stay in shared memory, and the
-// exact maximum and the sums travel through distributed shared memory.  Bound by its chain of phases.
+// exact maximum and the sums travel through distributed shared memory.  A warp's K blocks and then its
+// V blocks go through one ring, so V is on its way while the maxima are exchanged.  Bound by its chain of
+// phases.
 template <int HD, int GP>
 struct ClusterSmem {
   using T = Tile<HD, GP>;
+  using S = Slot<HD, GP, false>;
+  static constexpr int N = HD == 64 ? 4 : 3;     // ring slots
+  static constexpr int RING = DW * N * S::BYTES;
   static constexpr int TAIL = GP * HD + 2 * GP;  // this CTA's sums, maxima and weights for the cluster
-  static __host__ __device__ int64_t score_floats(int cap) { return cap * GP > T::PART ? cap * GP : T::PART; }
-  static size_t bytes(int cap) { return (score_floats(cap) + TAIL) * sizeof(float); }
+  static_assert(RING >= T::PART * 4, "the warps' sums take the rings' place");
+  static size_t bytes(int cap) { return RING + ((size_t)cap * GP + TAIL) * sizeof(float); }
 };
 
 template <int HD, int GP>
 __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1) decode_kv8_kernel(Kv8Attn a, int cap) {
   using T = Tile<HD, GP>;
+  using M = ClusterSmem<HD, GP>;
+  using S = Slot<HD, GP, false>;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), CL = (int)cluster.num_blocks();
   const int gk = blockIdx.y, b = blockIdx.z;
   const int G = a.n_heads / a.c.n_kv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  extern __shared__ __align__(16) float z[];                    // [NT][cap / 32] score blocks
-  float* pacc = z + ClusterSmem<HD, GP>::score_floats(cap);     // [GP][HD] this CTA's sums
-  float* stat = pacc + GP * HD;                                 // [GP] maximum, [GP] sum of weights
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* z = (float*)(smem + M::RING);   // [NT][cap / 32] score blocks
+  float* pacc = z + (int64_t)cap * GP;   // [GP][HD] this CTA's sums
+  float* stat = pacc + GP * HD;          // [GP] maximum, [GP] sum of weights
   __shared__ float wred[DW][GP], vred[DW], gmax[GP];
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -444,32 +498,40 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   const int per = ((len + CL - 1) / CL + 31) & ~31;
   const int j0 = min(len, rank * per), n = min(len - j0, per);
   const int64_t row0 = a.c.at(slot, gk, j0);
-  const int8_t* kp = a.c.k + row0 * HD;
-  const int8_t* vp = a.c.v + row0 * HD;
-  const float* ksp = a.c.ks + row0;
-  const float* vsp = a.c.vs + row0;
   const int64_t plane = (int64_t)cap * T::CP;
+  // the warp's blocks: K blocks warp, warp + DW, ..; then V blocks tw, tw + TW, ..
+  const int tw = warp / T::DS, d0 = (warp % T::DS) * T::DP;
+  const int blocks = (n + 31) >> 5;
+  const int nk = (blocks - warp + DW - 1) / DW, nv = (blocks - tw + T::TW - 1) / T::TW;
+  const uint8_t* ring = smem + warp * M::N * S::BYTES;
+  const uint32_t ring_at = smem_u32(ring);
+  const uint64_t policy = l2_evict_first_policy();
+  auto fetch = [&](int i) {
+    const uint32_t to = ring_at + i % M::N * S::BYTES;
+    if (i < nk)
+      S::fetch(to, a.c.k + row0 * HD, a.c.ks + row0, a.c.vs + row0, 32 * (warp + DW * i), n, lane, policy);
+    else if (i < nk + nv)
+      S::fetch(to, a.c.v + row0 * HD, nullptr, a.c.vs + row0, 32 * (tw + T::TW * (i - nk)), n, lane, policy);
+    cp_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < M::N - 1; ++i) fetch(i);
 
-  KBlock<HD> k;
-  if (32 * warp < n) k.load(kp, ksp, 32 * warp, n, g, t);
   float vmax = 0.f;
-  for (int j = tid; j < n; j += DT) vmax = max_nan(vmax, __ldg(vsp + j));
   uint32_t qd[T::NT][HD / 32][3][2];
   float unit[T::NT], mx[T::NT][2];
   load_q<HD, GP>(a.q + (int64_t)b * a.q_stride + (int64_t)gk * G * HD, a.q_vec, G, lane, qd, unit);
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
-  for (int row = 32 * warp; row < n; row += 32 * DW) {
-    score_block<HD, GP>(k, qd, g, t, z + (row >> 5) * T::ZB, plane, mx);
-    if (row + 32 * DW < n) k.load(kp, ksp, row + 32 * DW, n, g, t);
+  for (int i = 0; i < nk; ++i) {
+    cp_wait<M::N - 2>();
+    KBlock<HD> k;
+    S::read_k(ring + i % M::N * S::BYTES, k, vmax, lane);
+    fetch(i + M::N - 1);  // into the slot of block i - 1
+    score_block<HD, GP>(k, qd, g, t, z + (warp + DW * i) * T::ZB, plane, mx);
   }
-  // the warp's first V block travels while the maxima are exchanged
-  const int tw = warp / T::DS, d0 = (warp % T::DS) * T::DP;
-  VBlock<HD, GP> v;
-  if (32 * tw < n) v.load(vp, vsp, 32 * tw, n, lane, d0);
   warp_maxima<HD, GP>(mx, g, t, wred[warp]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) vmax = max_nan(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+  vmax = warp_max_nan(vmax);
   if (lane == 0) vred[warp] = vmax;
   __syncthreads();
   if (tid < GP) {
@@ -497,18 +559,23 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
     max_of[nt] = gmax[nt * 8 + col];
   }
   pv.start(vmax, max_of, unit);
-  for (int row = 32 * tw; row < n; row += 32 * T::TW) {
+  for (int i = nk; i < nk + nv; ++i) {
+    const int blk = tw + T::TW * (i - nk);
+    cp_wait<M::N - 2>();
+    VBlock<HD, GP> v;
+    S::read_v(ring + i % M::N * S::BYTES, v, n - 32 * blk, d0, lane);
+    fetch(i + M::N - 1);
     float zv[T::NT][pv.NZ];
 #pragma unroll
     for (int nt = 0; nt < T::NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < pv.NZ; i += 4)
-        *(float4*)&zv[nt][i] = *(const float4*)(z + nt * plane + (row >> 5) * T::ZB + pv.zstart(g, t) + i);
-    pv.add(v, zv, n - row, lane);
-    if (row + 32 * T::TW < n) v.load(vp, vsp, row + 32 * T::TW, n, lane, d0);
+      for (int c = 0; c < pv.NZ; c += 4)
+        *(float4*)&zv[nt][c] = *(const float4*)(z + nt * plane + blk * T::ZB + pv.zstart(g, t) + c);
+    pv.add(v, zv, n - 32 * blk, lane);
   }
-  __syncthreads();  // the scores are read
-  float* part = z;  // [TW][GP][HD]
+  cp_wait<0>();
+  __syncthreads();  // the rings are done
+  float* part = (float*)smem;  // [TW][GP][HD]
   pv.store(part + tw * GP * HD, wred[tw], lane, d0);
   __syncthreads();
   if (tid < GP) {
@@ -541,9 +608,8 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
 // Flat grids over chunks of keys, so that nothing waits inside a kernel: the scores of a chunk go to
 // global memory with the chunk's maxima (and its largest V scale), the second kernel reads them back
 // against the maximum over the chunks; the CTA that finishes a (sequence, kv head) joins its chunks'
-// sums, in order.  The scores add GP * 8 bytes to the 2 * HD + 8 of a key and mostly stay in L2.  Each warp streams its blocks through a ring of its
-// own (asynchronous copies, no barrier but the warp's), two or more blocks ahead of the one it works on.
-// Bound by HBM.
+// sums, in order.  The scores add GP * 8 bytes to the 2 * HD + 8 of a key and mostly stay in L2.  Bound by
+// HBM.
 struct Kv8Split {
   Kv8Attn a;
   int chunk, n_chunks;  // keys of a chunk (whole blocks); chunks that max_len makes
@@ -553,60 +619,22 @@ struct Kv8Split {
   float* pacc;          // [B][n_kv][n_chunks][GP][HD]
 };
 
-// 16-byte chunk c of row r of a block sits at c ^ swizzle(r): with it neither the K side (lanes of two
-// rows and 64 bytes at once) nor the V side (four rows, 32 bytes) meets a bank twice.
-template <int HD>
-__device__ __forceinline__ int swizzle(int r) {
-  return HD == 128 ? ((r & 1) << 2) | (r & 2) : r & 2;
-}
-
-// A warp's ring slot: codes of 32 rows, their V scales, then the K scales (scores) or the scores (P V).
 template <int HD, int GP, bool PV>
-struct Slot {
-  using T = Tile<HD, GP>;
-  static constexpr int CODES = 32 * HD;
-  static constexpr int MORE = CODES + 128;
-  static constexpr int BYTES = MORE + (PV ? T::NT * T::ZB * 4 : 128);
+struct SplitSmem {
+  using S = Slot<HD, GP, PV>;
   static constexpr int CTAS = PV ? ((GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1) : (GP == 16 ? 1 : 2);
-  // as many slots as the CTAs of an SM have room for, 3 at least
-  static constexpr int FIT = (CTAS == 2 ? 112 : 220) * 1024 / (DW * BYTES);
+  // as many slots as the CTAs of an SM have room for
+  static constexpr int FIT = (CTAS == 2 ? 112 : 220) * 1024 / (DW * S::BYTES);
   static constexpr int N = FIT > 6 ? 6 : FIT;
-  static constexpr int RING = DW * N * BYTES;
-  static_assert(N >= 3 && RING >= T::PART * 4, "ring too small");
-
-  // rows at or past n repeat row n - 1; ks only where the scores are formed
-  static __device__ __forceinline__ void fetch(uint32_t to, const int8_t* codes, const float* ks, const float* vs,
-                                               int row, int n, int lane, uint64_t policy) {
-    constexpr int C = HD / 16, R = 32 / C;  // chunks of a row; rows of 32 chunks
-    const int r = lane / C;
-    const uint32_t dst = to + r * HD + (((lane % C) ^ swizzle<HD>(r)) << 4);
-    const int8_t* src = codes + (int64_t)(row + r) * HD + (lane % C) * 16;
-    if (row + 32 <= n) {
-#pragma unroll
-      for (int j = 0; j < C; ++j) cp16_once(dst + j * 512, src + j * 512, policy);
-    } else {
-#pragma unroll
-      for (int j = 0; j < C; ++j) cp16_once(dst + j * 512, src + min(j * R, n - 1 - row - r) * HD, policy);
-    }
-    const int s = min(row + lane, n - 1);
-    cp4(to + CODES + 4 * lane, vs + s);
-    if (!PV) cp4(to + MORE + 4 * lane, ks + s);
-  }
-  // the block's scores, planes `plane` floats apart
-  static __device__ __forceinline__ void fetch_scores(uint32_t to, const float* z, int64_t plane, int row, int lane) {
-#pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < T::ZB / 128; ++j)
-        cp16(to + MORE + (nt * T::ZB + j * 128 + lane * 4) * 4,
-             z + nt * plane + (int64_t)(row >> 5) * T::ZB + j * 128 + lane * 4);
-  }
+  static constexpr int RING = DW * N * S::BYTES;
+  static_assert(N >= 3 && RING >= Tile<HD, GP>::PART * 4, "ring too small");
 };
 
 template <int HD, int GP>
-__global__ void __launch_bounds__(DT, (Slot<HD, GP, false>::CTAS)) split_scores_kernel(Kv8Split s) {
+__global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, false>::CTAS)) split_scores_kernel(Kv8Split s) {
   using T = Tile<HD, GP>;
   using S = Slot<HD, GP, false>;
+  using M = SplitSmem<HD, GP, false>;
   const Kv8Attn& a = s.a;
   const int ch = blockIdx.x, gk = blockIdx.y, b = blockIdx.z;
   const int G = a.n_heads / a.c.n_kv;
@@ -628,7 +656,7 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, false>::CTAS)) split_scores_
   const int64_t bg = (int64_t)b * a.c.n_kv + gk;
   const int64_t plane = (int64_t)s.n_chunks * s.chunk * T::CP;
   float* z = s.z + bg * T::NT * plane + (int64_t)(j0 >> 5) * T::ZB;
-  const uint8_t* ring = smem + warp * S::N * S::BYTES;
+  const uint8_t* ring = smem + warp * M::N * S::BYTES;
   const uint32_t ring_at = smem_u32(ring);
   const uint64_t policy = l2_evict_first_policy();
   // block i of the warp starts at row 32 (warp + DW i), slot i % N
@@ -637,7 +665,7 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, false>::CTAS)) split_scores_
     cp_commit();
   };
 #pragma unroll
-  for (int i = 0; i < S::N - 1; ++i) fetch(32 * (warp + DW * i), i);
+  for (int i = 0; i < M::N - 1; ++i) fetch(32 * (warp + DW * i), i);
   float vmax = 0.f;
   uint32_t qd[T::NT][HD / 32][3][2];
   float unit[T::NT], mx[T::NT][2];
@@ -646,27 +674,17 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, false>::CTAS)) split_scores_
   for (int nt = 0; nt < T::NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
   int at = 0;
   for (int row = 32 * warp; row < n; row += 32 * DW) {
-    cp_wait<S::N - 2>();
-    const uint8_t* p = ring + at * S::BYTES;
+    cp_wait<M::N - 2>();
     KBlock<HD> k;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int r = krow(g) + 4 * c;
-#pragma unroll
-      for (int l = 0; l < HD / 64; ++l)
-        *(uint4*)k.w[c][l] = *(const uint4*)(p + r * HD + (((l * 4 + t) ^ swizzle<HD>(g)) << 4));
-      k.s[c] = *(const float*)(p + S::MORE + 4 * r);
-    }
-    vmax = max_nan(vmax, *(const float*)(p + S::CODES + 4 * lane));
+    S::read_k(ring + at * S::BYTES, k, vmax, lane);
     // the slot of the block before this one is free
-    fetch(row + 32 * DW * (S::N - 1), at == 0 ? S::N - 1 : at - 1);
-    at = at == S::N - 1 ? 0 : at + 1;
+    fetch(row + 32 * DW * (M::N - 1), at == 0 ? M::N - 1 : at - 1);
+    at = at == M::N - 1 ? 0 : at + 1;
     score_block<HD, GP>(k, qd, g, t, z + (int64_t)(row >> 5) * T::ZB, plane, mx);
   }
   cp_wait<0>();
   warp_maxima<HD, GP>(mx, g, t, wred[warp]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) vmax = max_nan(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
+  vmax = warp_max_nan(vmax);
   if (lane == 0) vred[warp] = vmax;
   __syncthreads();
   float* stat = s.stat + (bg * s.n_chunks + ch) * (2 * GP + 1);
@@ -683,9 +701,10 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, false>::CTAS)) split_scores_
 }
 
 template <int HD, int GP>
-__global__ void __launch_bounds__(DT, (Slot<HD, GP, true>::CTAS)) split_pv_kernel(Kv8Split s) {
+__global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_kernel(Kv8Split s) {
   using T = Tile<HD, GP>;
   using S = Slot<HD, GP, true>;
+  using M = SplitSmem<HD, GP, true>;
   const Kv8Attn& a = s.a;
   const int ch = blockIdx.x, gk = blockIdx.y, b = blockIdx.z;
   const int G = a.n_heads / a.c.n_kv;
@@ -709,11 +728,11 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, true>::CTAS)) split_pv_kerne
   const int64_t plane = (int64_t)s.n_chunks * s.chunk * T::CP;
   const int tw = warp / T::DS, d0 = (warp % T::DS) * T::DP;
   const float* z = s.z + bg * T::NT * plane + (int64_t)(j0 >> 5) * T::ZB;
-  const uint8_t* ring = smem + warp * S::N * S::BYTES;
+  const uint8_t* ring = smem + warp * M::N * S::BYTES;
   const uint32_t ring_at = smem_u32(ring);
   const uint64_t policy = l2_evict_first_policy();
 #pragma unroll
-  for (int i = 0; i < S::N - 1; ++i)
+  for (int i = 0; i < M::N - 1; ++i)
     if (32 * (tw + T::TW * i) < n)
       S::fetch(ring_at + i * S::BYTES, vp, nullptr, vsp, 32 * (tw + T::TW * i), n, lane, policy);
   // the maximum over the sequence's chunks, and the factors of the heads
@@ -738,7 +757,7 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, true>::CTAS)) split_pv_kerne
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
 #pragma unroll
-  for (int i = 0; i < S::N - 1; ++i) {
+  for (int i = 0; i < M::N - 1; ++i) {
     const int row = 32 * (tw + T::TW * i);
     if (row < n) S::fetch_scores(ring_at + i * S::BYTES, z, plane, row, lane);
     cp_commit();  // the first group holds all of the codes so far
@@ -759,7 +778,7 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, true>::CTAS)) split_pv_kerne
   pv.start(vmax, max_of, unit);
   int at = 0;
   for (int row = 32 * tw; row < n; row += 32 * T::TW) {
-    cp_wait<S::N - 2>();
+    cp_wait<M::N - 2>();
     const uint8_t* p = ring + at * S::BYTES;
     float zv[T::NT][pv.NZ];
 #pragma unroll
@@ -768,24 +787,15 @@ __global__ void __launch_bounds__(DT, (Slot<HD, GP, true>::CTAS)) split_pv_kerne
       for (int i = 0; i < pv.NZ; i += 4)
         *(float4*)&zv[nt][i] = *((const float4*)(p + S::MORE) + (nt * T::ZB + pv.zstart(g, t) + i) / 4);
     VBlock<HD, GP> v;
-    v.s = row + lane < n ? *(const float*)(p + S::CODES + 4 * lane) : 0.f;
-    const int byte = d0 + g * T::VB;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint8_t* r = p + (t + 4 * i) * HD + (((byte >> 4) ^ swizzle<HD>(t)) << 4) + (byte & 15);
-      if constexpr (T::VB == 16)
-        *(uint4*)v.w[i] = *(const uint4*)r;
-      else
-        *(uint2*)v.w[i] = *(const uint2*)r;
-    }
-    const int next = row + 32 * T::TW * (S::N - 1);
+    S::read_v(p, v, n - row, d0, lane);
+    const int next = row + 32 * T::TW * (M::N - 1);
     if (next < n) {
-      const uint32_t to = ring_at + (at == 0 ? S::N - 1 : at - 1) * S::BYTES;
+      const uint32_t to = ring_at + (at == 0 ? M::N - 1 : at - 1) * S::BYTES;
       S::fetch(to, vp, nullptr, vsp, next, n, lane, policy);
       S::fetch_scores(to, z, plane, next, lane);
     }
     cp_commit();
-    at = at == S::N - 1 ? 0 : at + 1;
+    at = at == M::N - 1 ? 0 : at + 1;
     pv.add(v, zv, n - row, lane);
   }
   cp_wait<0>();
@@ -844,33 +854,66 @@ cudaLaunchConfig_t launch_config(dim3 grid, int threads, size_t smem, cudaStream
   return cfg;
 }
 
-// SM_ERR_UNSUPPORTED where the scores do not fit the cluster's shared memory.
+// How the cluster form would run, or size 0 where its scores do not fit or the split form is faster.
+//
+// Size: CTAs of one cluster have to be resident together, and a second wave of clusters waits for whole
+// groups of SMs, so the largest size is taken whose clusters are all resident at once (32 / 4 heads of 64,
+// 16 rows of up to 1024 keys: 4 CTAs 7.3 us, 8 CTAs, which are not, 13.2 us), with 128 keys a CTA at least
+// and none below 512 keys (b 1: at 128 keys 1 CTA 4.5 us, 4 CTAs 5.3 us; at 2048 keys 1 CTA 11.6 us, 16 CTAs
+// 5.8 us).  Split above 600 KB of codes an SM that has a CTA: at 262 KB (32 / 4 x 64, b 1, 32768 keys)
+// 13.4 us against 19.3 us split, at 1 MB (32 / 8 x 128, b 1, 32768 keys) 25.9 us against 24.6 us, at 2 MB
+// (16 / 16 x 128, b 1, 32768 keys) 51 us against 30 us.
+struct ClusterPlan {
+  int size, cap;
+  size_t smem;
+};
+
 template <int HD, int GP>
-int launch_decode_cluster(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st) {
-  using T = Tile<HD, GP>;
+int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan) {
+  using M = ClusterSmem<HD, GP>;
+  constexpr size_t HALF = 113 * 1024;  // of an SM's shared memory, so that two CTAs fit
   auto kern = decode_kv8_kernel<HD, GP>;
-  cudaLaunchAttribute attr[2];
-  // largest cluster that the device schedules (16 is not a portable size), found once
-  static int largest[64] = {};
+  // clusters of 1, 2, 4, 8, 16 CTAs resident at once, by CTAs of all the shared memory and of half of it
+  static int resident[64][2][5] = {};
+  static bool ready[64] = {};
   if (device >= 64) return fail(SM_ERR_UNSUPPORTED, "attention_kv8: device id too large");
-  if (!largest[device]) {
+  if (!ready[device]) {
     SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX));
     SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    cudaLaunchConfig_t probe = launch_config(dim3(16), DT, SMEM_MAX, st, 16, attr);
-    int fit = 0;
-    const bool ok = cudaOccupancyMaxActiveClusters(&fit, (const void*)kern, &probe) == cudaSuccess && fit > 0;
-    if (!ok) cudaGetLastError();
-    largest[device] = ok ? 16 : 8;
+    for (int half = 0; half < 2; ++half)
+      for (int i = 0; i < 5; ++i) {
+        cudaLaunchAttribute attr[2];
+        cudaLaunchConfig_t probe = launch_config(dim3(1 << i), DT, half ? HALF : SMEM_MAX, nullptr, 1 << i, attr);
+        int fit = 0;
+        if (cudaOccupancyMaxActiveClusters(&fit, (const void*)kern, &probe) != cudaSuccess) {
+          cudaGetLastError();
+          fit = 0;
+        }
+        resident[device][half][i] = fit;
+      }
+    ready[device] = true;
   }
-  int cl = largest[device];
-  while (cl > 1 && (int64_t)cl * a.c.n_kv * B > 2 * sms) cl >>= 1;
-  auto cap_of = [&](int c) { return ((a.max_len + c - 1) / c + 31) & ~31; };
-  while (cl < largest[device] && ClusterSmem<HD, GP>::bytes(cap_of(cl)) > SMEM_MAX) cl <<= 1;
-  if (getenv("CLX")) cl = atoi(getenv("CLX"));
-  const size_t smem = ClusterSmem<HD, GP>::bytes(cap_of(cl));
-  if (smem > SMEM_MAX) return SM_ERR_UNSUPPORTED;
-  const cudaLaunchConfig_t cfg = launch_config(dim3(cl, a.c.n_kv, B), DT, smem, st, cl, attr);
-  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a, cap_of(cl)));
+  const int64_t bg = (int64_t)B * a.c.n_kv;
+  plan.size = 0;
+  for (int i = 4; i >= 0; --i) {
+    const int cl = 1 << i;
+    if (cl > 1 && (a.max_len < 512 || cl * 128 > a.max_len)) continue;
+    const int cap = ((a.max_len + cl - 1) / cl + 31) & ~31;
+    const size_t smem = M::bytes(cap);
+    const int fit = resident[device][smem <= HALF][i];
+    if (smem > SMEM_MAX || (cl > 1 && bg > fit)) continue;
+    const int64_t codes = bg * a.max_len * 2 * HD, ctas = bg * cl;
+    if (codes / (ctas < sms ? ctas : sms) <= 600 * 1024) plan = {cl, cap, smem};
+    break;
+  }
+  return SM_OK;
+}
+
+template <int HD, int GP>
+int launch_decode_cluster(const Kv8Attn& a, int B, const ClusterPlan& plan, cudaStream_t st) {
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = launch_config(dim3(plan.size, a.c.n_kv, B), DT, plan.smem, st, plan.size, attr);
+  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, decode_kv8_kernel<HD, GP>, a, plan.cap));
   return SM_OK;
 }
 
@@ -878,8 +921,8 @@ template <int HD, int GP>
 int launch_decode_split(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st) {
   auto scores = split_scores_kernel<HD, GP>;
   auto pv = split_pv_kernel<HD, GP>;
-  using SK = Slot<HD, GP, false>;
-  using SV = Slot<HD, GP, true>;
+  using SK = SplitSmem<HD, GP, false>;
+  using SV = SplitSmem<HD, GP, true>;
   static bool ready[64] = {};
   if (device >= 64) return fail(SM_ERR_UNSUPPORTED, "attention_kv8: device id too large");
   if (!ready[device]) {
@@ -890,10 +933,10 @@ int launch_decode_split(const Kv8Attn& a, int B, int device, int sms, cudaStream
   Kv8Split s;
   s.a = a;
   const int64_t bg = (int64_t)B * a.c.n_kv;
-  const char* cx = getenv("CHX");
-  // one wave of CTAs where that makes chunks of at most 4096 keys
-  const int waves = (int)max((int64_t)1, (int64_t)SV::CTAS * sms / bg);
-  s.chunk = min(cx ? atoi(cx) : 2048, max(512, ((a.max_len + waves - 1) / waves + 31) & ~31));
+  // one wave of CTAs where that makes chunks of 512 to 4096 keys (b 1, 131071 keys, 32 / 8 x 128: chunks of
+  // 1024 keys 87 us, of 2048 72 us, one wave of 3552 68 us)
+  const int wave = (int)std::max<int64_t>(1, (int64_t)SV::CTAS * sms / bg);
+  s.chunk = std::min(4096, std::max(512, ((a.max_len + wave - 1) / wave + 31) & ~31));
   s.n_chunks = (a.max_len + s.chunk - 1) / s.chunk;
   const int64_t rows = bg * s.n_chunks;
   const int64_t nz = rows * s.chunk * GP, nstat = rows * (2 * GP + 1), nacc = rows * GP * HD;
@@ -919,13 +962,10 @@ int launch_decode_split(const Kv8Attn& a, int B, int device, int sms, cudaStream
 
 template <int HD, int GP>
 int launch_decode_as(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st, int* n_launch) {
-  const char* split = getenv("SPLITX");
-  if (!(split && split[0] == '1')) {
-    const int rc = launch_decode_cluster<HD, GP>(a, B, device, sms, st);
-    if (rc == SM_OK) *n_launch = 1;
-    if (rc != SM_ERR_UNSUPPORTED) return rc;
-  }
-  *n_launch = 2;
+  ClusterPlan plan;
+  SM_TRY((plan_cluster<HD, GP>(a, B, device, sms, plan)));
+  *n_launch = plan.size ? 1 : 2;
+  if (plan.size) return launch_decode_cluster<HD, GP>(a, B, plan, st);
   return launch_decode_split<HD, GP>(a, B, device, sms, st);
 }
 
@@ -971,15 +1011,15 @@ bool q_rows_vec(const float* q, int64_t q_stride) { return (uintptr_t)q % 16 == 
 
 int check_attn(sm_ctx* ctx, const sm_kv8* c, const float* q, int64_t q_stride, const int* seq_ids, const int* lens,
                int max_len, int B, int n_heads, const float* out, const char* what) {
-  const std::string w(what);
+  auto refuse = [&](int code, const char* why) { return fail(code, std::string(what) + ": " + why); };
   SM_TRY(kv8_check(c, what));
-  if (B < 0 || n_heads <= 0 || n_heads % c->n_kv) return fail(SM_ERR_SHAPE, w + ": bad shape");
-  if (n_heads / c->n_kv > 16) return fail(SM_ERR_UNSUPPORTED, w + ": more than 16 q heads per kv head");
-  if (max_len < 0 || max_len > c->max_tokens) return fail(SM_ERR_SHAPE, w + ": max_len outside 0 .. max_tokens");
-  if (q_stride < (int64_t)n_heads * c->head_dim) return fail(SM_ERR_SHAPE, w + ": q_stride is less than a row");
-  if (!seq_ids && B > c->max_seqs) return fail(SM_ERR_SHAPE, w + ": more rows than slots");
-  if (!ctx || (B && (!q || !lens || !out))) return fail(SM_ERR_INVALID_ARG, w + ": null argument");
-  if (((uintptr_t)q | (uintptr_t)out) % 4) return fail(SM_ERR_INVALID_ARG, w + ": misaligned pointer");
+  if (B < 0 || n_heads <= 0 || n_heads % c->n_kv) return refuse(SM_ERR_SHAPE, "bad shape");
+  if (n_heads / c->n_kv > 16) return refuse(SM_ERR_UNSUPPORTED, "more than 16 q heads per kv head");
+  if (max_len < 0 || max_len > c->max_tokens) return refuse(SM_ERR_SHAPE, "max_len outside 0 .. max_tokens");
+  if (q_stride < (int64_t)n_heads * c->head_dim) return refuse(SM_ERR_SHAPE, "q_stride is less than a row");
+  if (!seq_ids && B > c->max_seqs) return refuse(SM_ERR_SHAPE, "more rows than slots");
+  if (!ctx || (B && (!q || !lens || !out))) return refuse(SM_ERR_INVALID_ARG, "null argument");
+  if (((uintptr_t)q | (uintptr_t)out) % 4) return refuse(SM_ERR_INVALID_ARG, "misaligned pointer");
   return SM_OK;
 }
 

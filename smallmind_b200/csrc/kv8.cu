@@ -1,7 +1,7 @@
 // Writing and reading the 8-bit KV cache.
 //
 // A head's row x[hd] is kept as codes c and one scale s:
-//   s = fl32(max|x| / 127),  c = x / s rounded to the nearest integer (ties to even),
+//   s = fl32(max|x| * fl32(1 / 127)),  c = x / s rounded to the nearest integer (ties to even),
 // and read back as fl32(c * s).  The rounding is exact: with q the candidate next to
 // x * (1 / s), the remainder r = x - q * s is formed without error by one FMA (q has 7
 // bits and |r| <= ~s, so r fits 24 bits), and q stands unless |r| >= s / 2.  That test
@@ -17,15 +17,15 @@
 namespace sm {
 
 int kv8_check(const sm_kv8* c, const char* what) {
-  const std::string w(what);
-  if (!c) return fail(SM_ERR_INVALID_ARG, w + ": null cache");
-  if (c->max_seqs <= 0 || c->max_tokens <= 0 || c->n_kv <= 0) return fail(SM_ERR_SHAPE, w + ": bad cache shape");
-  if (c->head_dim != 64 && c->head_dim != 128) return fail(SM_ERR_UNSUPPORTED, w + ": head_dim must be 64 or 128");
-  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(SM_ERR_INVALID_ARG, w + ": null cache array");
+  auto refuse = [&](int code, const char* why) { return fail(code, std::string(what) + ": " + why); };
+  if (!c) return refuse(SM_ERR_INVALID_ARG, "null cache");
+  if (c->max_seqs <= 0 || c->max_tokens <= 0 || c->n_kv <= 0) return refuse(SM_ERR_SHAPE, "bad cache shape");
+  if (c->head_dim != 64 && c->head_dim != 128) return refuse(SM_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
+  if (!c->k || !c->v || !c->k_scale || !c->v_scale) return refuse(SM_ERR_INVALID_ARG, "null cache array");
   if (((uintptr_t)c->k | (uintptr_t)c->v) % 16)
-    return fail(SM_ERR_INVALID_ARG, w + ": the code arrays must be 16-byte aligned");
+    return refuse(SM_ERR_INVALID_ARG, "the code arrays must be 16-byte aligned");
   if (((uintptr_t)c->k_scale | (uintptr_t)c->v_scale) % 4)
-    return fail(SM_ERR_INVALID_ARG, w + ": the scale arrays must be 4-byte aligned");
+    return refuse(SM_ERR_INVALID_ARG, "the scale arrays must be 4-byte aligned");
   return SM_OK;
 }
 
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(THREADS) kv8_write_kernel(Kv8View c, const flo
   for (int o = LANES / 2; o > 0; o >>= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
   if (!live) return;
   uint32_t word = 0;
-  float s = __fdiv_rn(__int_as_float(peak), 127.f);
+  float s = __int_as_float(peak) * (1.f / 127.f);
   if (peak >= 0x7f800000)
     s = __int_as_float(0x7fffffff);
   else if (s > 0.f)
@@ -149,11 +149,11 @@ __global__ void __launch_bounds__(THREADS) kv8_read_kernel(Kv8View c, const int*
 
 int check_rows(sm_ctx* ctx, const sm_kv8* c, const int* seq_ids, const int* positions, int n_rows, int64_t row_stride,
                const char* what) {
-  const std::string w(what);
+  auto refuse = [&](int code, const char* why) { return fail(code, std::string(what) + ": " + why); };
   SM_TRY(kv8_check(c, what));
-  if (n_rows < 0) return fail(SM_ERR_SHAPE, w + ": n_rows must not be negative");
-  if (row_stride < (int64_t)c->n_kv * c->head_dim) return fail(SM_ERR_SHAPE, w + ": row_stride is less than a row");
-  if (!ctx || (n_rows && (!seq_ids || !positions))) return fail(SM_ERR_INVALID_ARG, w + ": null argument");
+  if (n_rows < 0) return refuse(SM_ERR_SHAPE, "n_rows must not be negative");
+  if (row_stride < (int64_t)c->n_kv * c->head_dim) return refuse(SM_ERR_SHAPE, "row_stride is less than a row");
+  if (!ctx || (n_rows && (!seq_ids || !positions))) return refuse(SM_ERR_INVALID_ARG, "null argument");
   return SM_OK;
 }
 

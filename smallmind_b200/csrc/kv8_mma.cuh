@@ -78,16 +78,6 @@ __device__ __forceinline__ float kv8_weight(float x) {
   return fmaf(6.f, c, a) * r;
 }
 
-// 16 / 8 bytes of codes that are read once
-__device__ __forceinline__ void ld_codes(const int8_t* p, uint32_t (&w)[4]) {
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-               : "l"(p));
-}
-__device__ __forceinline__ void ld_codes(const int8_t* p, uint32_t (&w)[2]) {
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
-}
-
 // Asynchronous copies into shared memory, in groups that a warp waits for itself
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");

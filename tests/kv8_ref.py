@@ -3,11 +3,12 @@ import numpy as np
 
 
 def quantize(x):
-    """x [..., hd] fp32 -> (codes int8, scales fp32): scale = max|x| / 127, codes rounded half to even."""
+    """x [..., hd] fp32 -> (codes int8, scales fp32): scale = max|x| * (1 / 127) in fp32, codes rounded half to
+    even."""
     x = np.asarray(x, np.float32)
     peak = np.abs(x).max(-1)
     bad = ~np.isfinite(peak)
-    scale = (np.where(bad, 0, peak).astype(np.float64) / 127.0).astype(np.float32)
+    scale = np.where(bad, 0, peak).astype(np.float32) * np.float32(1 / 127)
     s = np.where(scale > 0, scale, 1).astype(np.float64)[..., None]
     q = np.rint(np.where(bad[..., None], 0, x).astype(np.float64) / s)
     codes = np.where((scale > 0)[..., None], np.clip(q, -127, 127), 0).astype(np.int8)
