@@ -836,24 +836,6 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
 
 constexpr size_t SMEM_MAX = 220 * 1024;
 
-cudaLaunchConfig_t launch_config(dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster,
-                                 cudaLaunchAttribute (&attr)[2]) {
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = cluster;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cfg;
-}
-
 // How the cluster form would run, or size 0 where its scores do not fit or the split form is faster.
 //
 // Size: CTAs of one cluster have to be resident together, and a second wave of clusters waits for whole

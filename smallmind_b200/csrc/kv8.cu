@@ -8,10 +8,10 @@
 // fails only for values within an ulp or so of a border, which then take a float64
 // division.  So the codes do not depend on how the quotient was formed.
 //
-// Both kernels are bound by HBM: a write moves 4 + 1 bytes a value and 4 a scale, a read
-// the same.  A lane takes 4 neighbouring values (16 bytes of fp32, 4 of codes), a head's
-// row sits in hd / 4 lanes of one warp, so the maximum is a few shuffles and every load
-// and store of a warp is contiguous.
+// Both kernels are bound by HBM: a write moves 4 + 1 bytes a value and 4 a scale, a read the same.  A lane
+// takes 4 neighbouring values (16 bytes of fp32, 4 of codes), so every access of a warp is contiguous and a
+// head's maximum is one reduction over its 16 or 32 lanes.  What hides the latency is bytes on their way: a
+// warp takes several pieces of 128 values and starts all of their loads before it uses the first.
 #include "kv8.cuh"
 
 namespace sm {
@@ -33,17 +33,12 @@ namespace {
 
 constexpr int THREADS = 256;
 
-// Slot and position of row i, or false where the row is padding or out of range.
-__device__ __forceinline__ bool row_target(const int* seq_ids, const int* positions, int64_t i, const Kv8View& c,
-                                           int* status, int& slot, int& pos) {
-  slot = seq_ids[i];
+// Whether a row is neither padding nor out of range
+__device__ __forceinline__ bool in_cache(const Kv8View& c, int slot, int pos, int* status) {
   if (slot < 0) return false;
-  pos = positions[i];
-  if (slot >= c.slots || pos < 0 || pos >= c.tokens) {
-    atomicExch(status, SM_ERR_SHAPE);
-    return false;
-  }
-  return true;
+  if (slot < c.slots && pos >= 0 && pos < c.tokens) return true;
+  atomicExch(status, SM_ERR_SHAPE);
+  return false;
 }
 
 __device__ __forceinline__ int code64(float x, float s) {
@@ -54,7 +49,7 @@ __device__ __forceinline__ int code64(float x, float s) {
 // Codes of four values under scale s, packed into a word (value 0 in the low byte).
 __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float s) {
   const float MAGIC = 12582912.f;  // 1.5 * 2^23: adding it leaves the rounded integer in the low mantissa bits
-  const float inv = 1.f / s, half = 0.5f * s;
+  const float inv = __fdividef(1.f, s), half = 0.5f * s;  // an approximate quotient: the remainder decides
   uint32_t bits[4];
   bool near_border = s < 1e-30f;  // where s / 2 or 1 / s might round
 #pragma unroll
@@ -71,81 +66,118 @@ __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float s) {
   return __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
 }
 
-// Item (row, K | V, head), head fastest.  HD / 4 lanes an item.
-template <int HD, bool VEC>
+// A warp's share: N pieces of 128 values, from piece N * (blockIdx.y / 2), of the K (even blockIdx.y) or V
+// values of row blockIdx.x * warps + warp.  Both sides are walked by constant steps.
+template <int HD, int N>
+struct Share {
+  int row, value, dim, left;  // row; this lane's first value in it; its dim; values from it to the row's end
+  int64_t step;               // from a piece's place in the cache to the next one's, in positions
+  bool is_v;
+  __device__ __forceinline__ Share(const Kv8View& c) {
+    const int lane = threadIdx.x % 32;
+    row = blockIdx.x * (THREADS / 32) + threadIdx.x / 32;
+    is_v = blockIdx.y & 1;
+    value = (int)(blockIdx.y >> 1) * (N * 128) + 4 * lane;
+    dim = value % HD;
+    left = c.n_kv * HD - value;
+    step = (int64_t)c.tokens * (128 / HD);
+  }
+  // this lane's place in the cache: position and head of its first value
+  __device__ __forceinline__ int64_t at(const Kv8View& c, int slot, int pos) const {
+    return c.at(slot, value / HD, pos);
+  }
+};
+
+template <int HD, int N, bool VEC>
 __global__ void __launch_bounds__(THREADS) kv8_write_kernel(Kv8View c, const float* __restrict__ k,
                                                             const float* __restrict__ v, int64_t row_stride,
                                                             const int* __restrict__ seq_ids,
-                                                            const int* __restrict__ positions, int64_t n_items,
+                                                            const int* __restrict__ positions, int n_rows,
                                                             int* status) {
-  constexpr int LANES = HD / 4;
-  const int lane = threadIdx.x % LANES;
-  const int64_t item = (int64_t)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
-  int slot = 0, pos = 0, head = 0;
-  bool is_v = false, live = false;
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (item < n_items) {
-    const int64_t row = item / (2 * c.n_kv);
-    head = (int)(item - row * (2 * c.n_kv));
-    is_v = head >= c.n_kv;
-    if (is_v) head -= c.n_kv;
-    live = row_target(seq_ids, positions, row, c, status, slot, pos);
-    if (live) {
-      const float* src = (is_v ? v : k) + row * row_stride + head * HD + 4 * lane;
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Share<HD, N> w(c);
+  if (w.row >= n_rows) return;
+  const int slot = __ldg(seq_ids + w.row), pos = __ldg(positions + w.row);
+  const float* src = (w.is_v ? v : k) + w.row * row_stride + w.value;
+  float x[N][4];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
+    if (w.left > i * 128) {
       if (VEC) {
-        const float4 t = *(const float4*)src;
-        x[0] = t.x, x[1] = t.y, x[2] = t.z, x[3] = t.w;
+        *(float4*)x[i] = __ldcs((const float4*)(src + i * 128));
       } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = src[i];
+        for (int e = 0; e < 4; ++e) x[i][e] = src[i * 128 + e];
       }
     }
   }
-  // the maximum as bits: non-negative floats order like integers, and infinities and NaNs lie above them
-  int peak = 0;
+  if (!in_cache(c, slot, pos, status)) return;
+  const int64_t at = w.at(c, slot, pos);
+  int8_t* codes = (w.is_v ? c.v : c.k) + at * HD + w.dim;
+  float* scales = (w.is_v ? c.vs : c.ks) + at;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) peak = max(peak, __float_as_int(x[i]) & 0x7fffffff);
+  for (int i = 0; i < N; ++i) {
+    // the maximum as bits: non-negative floats order like integers, and infinities and NaNs lie above them
+    unsigned peak = 0;
 #pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) peak = max(peak, __shfl_xor_sync(0xffffffffu, peak, o));
-  if (!live) return;
-  uint32_t word = 0;
-  float s = __int_as_float(peak) * (1.f / 127.f);
-  if (peak >= 0x7f800000)
-    s = __int_as_float(0x7fffffff);
-  else if (s > 0.f)
-    word = codes4(x, s);
-  const int64_t at = c.at(slot, head, pos);
-  *(uint32_t*)((is_v ? c.v : c.k) + at * HD + 4 * lane) = word;
-  if (lane == 0) (is_v ? c.vs : c.ks)[at] = s;
-}
-
-template <int HD, bool VEC>
-__global__ void __launch_bounds__(THREADS) kv8_read_kernel(Kv8View c, const int* __restrict__ seq_ids,
-                                                           const int* __restrict__ positions, int64_t n_items,
-                                                           float* __restrict__ k, float* __restrict__ v,
-                                                           int64_t row_stride, int* status) {
-  constexpr int LANES = HD / 4;
-  const int lane = threadIdx.x % LANES;
-  const int64_t item = (int64_t)blockIdx.x * (THREADS / LANES) + threadIdx.x / LANES;
-  if (item >= n_items) return;
-  const int64_t row = item / (2 * c.n_kv);
-  int head = (int)(item - row * (2 * c.n_kv));
-  const bool is_v = head >= c.n_kv;
-  if (is_v) head -= c.n_kv;
-  float* to = is_v ? v : k;
-  int slot, pos;
-  if (!to || !row_target(seq_ids, positions, row, c, status, slot, pos)) return;
-  const int64_t at = c.at(slot, head, pos);
-  const char4 w = *(const char4*)((is_v ? c.v : c.k) + at * HD + 4 * lane);
-  const float s = (is_v ? c.vs : c.ks)[at];
-  to += row * row_stride + head * HD + 4 * lane;
-  const float4 y = make_float4((float)w.x * s, (float)w.y * s, (float)w.z * s, (float)w.w * s);
-  if (VEC) {
-    *(float4*)to = y;
-  } else {
-    to[0] = y.x, to[1] = y.y, to[2] = y.z, to[3] = y.w;
+    for (int e = 0; e < 4; ++e) peak = max(peak, __float_as_uint(x[i][e]) & 0x7fffffffu);
+    peak = __reduce_max_sync(HD == 128 ? 0xffffffffu : threadIdx.x % 32 < 16 ? 0xffffu : 0xffff0000u, peak);
+    if (w.left > i * 128) {
+      uint32_t word = 0;
+      float s = __uint_as_float(peak) * (1.f / 127.f);
+      if (peak >= 0x7f800000u)
+        s = __uint_as_float(0x7fffffffu);
+      else if (s > 0.f)
+        word = codes4(x[i], s);
+      *(uint32_t*)codes = word;
+      if (w.dim == 0) *scales = s;
+    }
+    codes += w.step * HD;
+    scales += w.step;
   }
 }
+
+template <int HD, int N, bool VEC>
+__global__ void __launch_bounds__(THREADS) kv8_read_kernel(Kv8View c, const int* __restrict__ seq_ids,
+                                                           const int* __restrict__ positions, int n_rows,
+                                                           float* __restrict__ k, float* __restrict__ v,
+                                                           int64_t row_stride, int* status) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Share<HD, N> w(c);
+  float* to = w.is_v ? v : k;
+  if (w.row >= n_rows || !to) return;
+  const int slot = __ldg(seq_ids + w.row), pos = __ldg(positions + w.row);
+  if (!in_cache(c, slot, pos, status)) return;
+  const int64_t at = w.at(c, slot, pos);
+  const int8_t* codes = (w.is_v ? c.v : c.k) + at * HD + w.dim;
+  const float* scales = (w.is_v ? c.vs : c.ks) + at;
+  char4 q[N];
+  float s[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (w.left > i * 128) {
+      q[i] = *(const char4*)(codes + i * w.step * HD);
+      s[i] = scales[i * w.step];
+    }
+  to += w.row * row_stride + w.value;
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (w.left > i * 128) {
+      const float4 y = make_float4((float)q[i].x * s[i], (float)q[i].y * s[i], (float)q[i].z * s[i], (float)q[i].w * s[i]);
+      if (VEC) {
+        __stcs((float4*)(to + i * 128), y);
+      } else {
+        to[i * 128] = y.x, to[i * 128 + 1] = y.y, to[i * 128 + 2] = y.z, to[i * 128 + 3] = y.w;
+      }
+    }
+}
+
+// Pieces a warp takes: all of a row's up to 4.
+inline int share_of(int pieces) { return pieces >= 3 ? 4 : pieces; }
 
 int check_rows(sm_ctx* ctx, const sm_kv8* c, const int* seq_ids, const int* positions, int n_rows, int64_t row_stride,
                const char* what) {
@@ -179,14 +211,18 @@ SM_API int sm_kv8_write(sm_ctx* ctx, const sm_kv8* cache, const float* k, const 
   SM_TRY(ctx_view(ctx, &device, &st, &launches));
   DeviceGuard guard(device);
   const Kv8View c = kv8_view(cache);
-  const int64_t items = (int64_t)n_rows * 2 * c.n_kv;
-  const int64_t grid = (items * (cache->head_dim / 4) + THREADS - 1) / THREADS;
-  if (grid > INT32_MAX) return fail(SM_ERR_SHAPE, "kv8_write: too many rows");
+  const int pieces = ceil_div((int64_t)c.n_kv * cache->head_dim, 128), n = share_of(pieces);
+  const dim3 grid(ceil_div(n_rows, THREADS / 32), 2 * ceil_div(pieces, n));
   const bool vec = rows_vectorizable(k, v, row_stride);
-  auto kern = cache->head_dim == 64 ? (vec ? kv8_write_kernel<64, true> : kv8_write_kernel<64, false>)
-                                    : (vec ? kv8_write_kernel<128, true> : kv8_write_kernel<128, false>);
-  kern<<<(int)grid, THREADS, 0, st>>>(c, k, v, row_stride, seq_ids, positions, items, ctx_status(ctx));
-  SM_CUDA_TRY(cudaGetLastError());
+  const int which = (cache->head_dim == 64 ? 0 : 6) + (n == 4 ? 4 : 2 * (n - 1)) + vec;
+  decltype(&kv8_write_kernel<64, 1, false>) const kernels[] = {
+      kv8_write_kernel<64, 1, false>,  kv8_write_kernel<64, 1, true>,  kv8_write_kernel<64, 2, false>,
+      kv8_write_kernel<64, 2, true>,   kv8_write_kernel<64, 4, false>, kv8_write_kernel<64, 4, true>,
+      kv8_write_kernel<128, 1, false>, kv8_write_kernel<128, 1, true>, kv8_write_kernel<128, 2, false>,
+      kv8_write_kernel<128, 2, true>,  kv8_write_kernel<128, 4, false>, kv8_write_kernel<128, 4, true>};
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = launch_config(grid, THREADS, 0, st, 1, attr);
+  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernels[which], c, k, v, row_stride, seq_ids, positions, n_rows, ctx_status(ctx)));
   *launches += 1;
   return SM_OK;
 }
@@ -202,14 +238,18 @@ SM_API int sm_kv8_read(sm_ctx* ctx, const sm_kv8* cache, const int* seq_ids, con
   SM_TRY(ctx_view(ctx, &device, &st, &launches));
   DeviceGuard guard(device);
   const Kv8View c = kv8_view(cache);
-  const int64_t items = (int64_t)n_rows * 2 * c.n_kv;
-  const int64_t grid = (items * (cache->head_dim / 4) + THREADS - 1) / THREADS;
-  if (grid > INT32_MAX) return fail(SM_ERR_SHAPE, "kv8_read: too many rows");
+  const int pieces = ceil_div((int64_t)c.n_kv * cache->head_dim, 128), n = share_of(pieces);
+  const dim3 grid(ceil_div(n_rows, THREADS / 32), 2 * ceil_div(pieces, n));
   const bool vec = rows_vectorizable(k, v, row_stride);
-  auto kern = cache->head_dim == 64 ? (vec ? kv8_read_kernel<64, true> : kv8_read_kernel<64, false>)
-                                    : (vec ? kv8_read_kernel<128, true> : kv8_read_kernel<128, false>);
-  kern<<<(int)grid, THREADS, 0, st>>>(c, seq_ids, positions, items, k, v, row_stride, ctx_status(ctx));
-  SM_CUDA_TRY(cudaGetLastError());
+  const int which = (cache->head_dim == 64 ? 0 : 6) + (n == 4 ? 4 : 2 * (n - 1)) + vec;
+  decltype(&kv8_read_kernel<64, 1, false>) const kernels[] = {
+      kv8_read_kernel<64, 1, false>,  kv8_read_kernel<64, 1, true>,  kv8_read_kernel<64, 2, false>,
+      kv8_read_kernel<64, 2, true>,   kv8_read_kernel<64, 4, false>, kv8_read_kernel<64, 4, true>,
+      kv8_read_kernel<128, 1, false>, kv8_read_kernel<128, 1, true>, kv8_read_kernel<128, 2, false>,
+      kv8_read_kernel<128, 2, true>,  kv8_read_kernel<128, 4, false>, kv8_read_kernel<128, 4, true>};
+  cudaLaunchAttribute attr[2];
+  const cudaLaunchConfig_t cfg = launch_config(grid, THREADS, 0, st, 1, attr);
+  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernels[which], c, seq_ids, positions, n_rows, k, v, row_stride, ctx_status(ctx)));
   *launches += 1;
   return SM_OK;
 }

@@ -24,4 +24,24 @@ inline Kv8View kv8_view(const sm_kv8* c) {
   return {c->k, c->v, c->k_scale, c->v_scale, c->max_seqs, c->max_tokens, c->n_kv};
 }
 
+// Launch on a stream after its previous kernel by programmatic dependent launch: the kernel waits
+// (griddepcontrol.wait) before it touches memory.  attr backs the result.
+inline cudaLaunchConfig_t launch_config(dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster,
+                                 cudaLaunchAttribute (&attr)[2]) {
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cfg;
+}
+
 }  // namespace sm
