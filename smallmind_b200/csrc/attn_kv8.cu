@@ -399,10 +399,10 @@ struct Slot {
     const int8_t* src = codes + (int64_t)(row + r) * HD + (lane % C) * 16;
     if (row + 32 <= n) {
 #pragma unroll
-      for (int j = 0; j < C; ++j) cp16_once(dst + j * 512, src + j * 512, policy);
+      for (int j = 0; j < C; ++j) cp16(dst + j * 512, src + j * 512, policy);
     } else {
 #pragma unroll
-      for (int j = 0; j < C; ++j) cp16_once(dst + j * 512, src + min(j * R, n - 1 - row - r) * HD, policy);
+      for (int j = 0; j < C; ++j) cp16(dst + j * 512, src + min(j * R, n - 1 - row - r) * HD, policy);
     }
     const int s = min(row + lane, n - 1);
     cp4(to + CODES + 4 * lane, vs + s);
@@ -453,7 +453,7 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 
 // ---------------------------------------------------------------- decode, short: one cluster per (sequence, kv head)
 //
-// One launch: the keys are split over the cluster's CTAs, the scores stay in shared memory, and the
+// One launch: the keys (a shared prefix's blocks first, then the sequence's own) are split over the cluster's CTAs, the scores stay in shared memory, and the
 // exact maximum and the sums travel through distributed shared memory.  A warp's K blocks and then its
 // V blocks go through one ring, so V is on its way while the maxima are exchanged.  Bound by its chain of
 // phases.
@@ -465,7 +465,7 @@ struct ClusterSmem {
   static constexpr int RING = DW * N * S::BYTES;
   static constexpr int TAIL = GP * HD + 2 * GP;  // this CTA's sums, maxima and weights for the cluster
   static_assert(RING >= T::PART * 4, "the warps' sums take the rings' place");
-  static size_t bytes(int cap) { return RING + ((size_t)cap * GP + TAIL) * sizeof(float); }
+  static size_t bytes(int64_t cap) { return RING + ((size_t)cap * GP + TAIL) * sizeof(float); }
 };
 
 template <int HD, int GP>
@@ -489,29 +489,38 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   int slot, len;
   if (!row_keys(a, b, slot, len)) return;
   float* out = a.out + ((int64_t)b * a.n_heads + gk * G) * HD;
-  if (len == 0) {
+  if (a.prefix_len + len == 0) {
     if (rank == 0)
       for (int i = tid; i < G * HD; i += DT) out[i] = 0.f;
     return;
   }
-  // this CTA's keys: whole blocks
-  const int per = ((len + CL - 1) / CL + 31) & ~31;
-  const int j0 = min(len, rank * per), n = min(len - j0, per);
-  const int64_t row0 = a.c.at(slot, gk, j0);
+  // this CTA's blocks of all: the prefix's np, then the sequence's own
+  const int np = (a.prefix_len + 31) >> 5, all = np + ((len + 31) >> 5);
+  const int per = (all + CL - 1) / CL;
+  const int b0 = min(all, rank * per), blocks = min(all - b0, per);
+  const int64_t own0 = a.c.at(slot, gk, 0), prefix0 = a.prefix.at(a.prefix_seq, gk, 0);
   const int64_t plane = (int64_t)cap * T::CP;
+  // keys of a block
+  auto keys_of = [&](int blk) {
+    const int i = b0 + blk;
+    return i < np ? a.prefix_len - 32 * i : len - 32 * (i - np);
+  };
   // the warp's blocks: K blocks warp, warp + DW, ..; then V blocks tw, tw + TW, ..
   const int tw = warp / T::DS, d0 = (warp % T::DS) * T::DP;
-  const int blocks = (n + 31) >> 5;
   const int nk = (blocks - warp + DW - 1) / DW, nv = (blocks - tw + T::TW - 1) / T::TW;
   const uint8_t* ring = smem + warp * M::N * S::BYTES;
   const uint32_t ring_at = smem_u32(ring);
-  const uint64_t policy = l2_evict_first_policy();
+  const uint64_t once = l2_evict_first_policy(), often = l2_evict_normal_policy();
   auto fetch = [&](int i) {
-    const uint32_t to = ring_at + i % M::N * S::BYTES;
-    if (i < nk)
-      S::fetch(to, a.c.k + row0 * HD, a.c.ks + row0, a.c.vs + row0, 32 * (warp + DW * i), n, lane, policy);
-    else if (i < nk + nv)
-      S::fetch(to, a.c.v + row0 * HD, nullptr, a.c.vs + row0, 32 * (tw + T::TW * (i - nk)), n, lane, policy);
+    if (i < nk + nv) {
+      const bool is_k = i < nk;
+      const int blk = b0 + (is_k ? warp + DW * i : tw + T::TW * (i - nk));
+      const bool shared = blk < np;
+      const Kv8View& c = shared ? a.prefix : a.c;
+      const int64_t row0 = shared ? prefix0 : own0;
+      S::fetch(ring_at + i % M::N * S::BYTES, (is_k ? c.k : c.v) + row0 * HD, is_k ? c.ks + row0 : nullptr, c.vs + row0,
+               32 * (shared ? blk : blk - np), shared ? a.prefix_len : len, lane, shared ? often : once);
+    }
     cp_commit();
   };
 #pragma unroll
@@ -563,7 +572,7 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
     const int blk = tw + T::TW * (i - nk);
     cp_wait<M::N - 2>();
     VBlock<HD, GP> v;
-    S::read_v(ring + i % M::N * S::BYTES, v, n - 32 * blk, d0, lane);
+    S::read_v(ring + i % M::N * S::BYTES, v, keys_of(blk), d0, lane);
     fetch(i + M::N - 1);
     float zv[T::NT][pv.NZ];
 #pragma unroll
@@ -571,7 +580,7 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
 #pragma unroll
       for (int c = 0; c < pv.NZ; c += 4)
         *(float4*)&zv[nt][c] = *(const float4*)(z + nt * plane + blk * T::ZB + pv.zstart(g, t) + c);
-    pv.add(v, zv, n - 32 * blk, lane);
+    pv.add(v, zv, keys_of(blk), lane);
   }
   cp_wait<0>();
   __syncthreads();  // the rings are done
@@ -876,16 +885,17 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
     ready[device] = true;
   }
   const int64_t bg = (int64_t)B * a.c.n_kv;
+  const int64_t blocks = ((int64_t)a.prefix_len + 31) / 32 + ((int64_t)a.max_len + 31) / 32, keys = 32 * blocks;
   plan.size = 0;
   for (int i = 4; i >= 0; --i) {
     const int cl = 1 << i;
-    if (cl > 1 && (a.max_len < 512 || cl * 128 > a.max_len)) continue;
-    const int cap = ((a.max_len + cl - 1) / cl + 31) & ~31;
+    if (cl > 1 && (keys < 512 || cl * 128 > keys)) continue;
+    const int64_t cap = 32 * ((blocks + cl - 1) / cl);
     const size_t smem = M::bytes(cap);
     const int fit = resident[device][smem <= HALF][i];
     if (smem > SMEM_MAX || (cl > 1 && bg > fit)) continue;
-    const int64_t codes = bg * a.max_len * 2 * HD, ctas = bg * cl;
-    if (codes / (ctas < sms ? ctas : sms) <= 600 * 1024) plan = {cl, cap, smem};
+    const int64_t codes = bg * keys * 2 * HD, ctas = bg * cl;
+    if (codes / (ctas < sms ? ctas : sms) <= 600 * 1024) plan = {cl, (int)cap, smem};
     break;
   }
   return SM_OK;
@@ -946,8 +956,9 @@ template <int HD, int GP>
 int launch_decode_as(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st, int* n_launch) {
   ClusterPlan plan;
   SM_TRY((plan_cluster<HD, GP>(a, B, device, sms, plan)));
-  *n_launch = plan.size ? 1 : 2;
+  *n_launch = plan.size ? 1 : a.prefix.k ? 0 : 2;
   if (plan.size) return launch_decode_cluster<HD, GP>(a, B, plan, st);
+  if (a.prefix.k) return SM_OK;
   return launch_decode_split<HD, GP>(a, B, device, sms, st);
 }
 
@@ -971,11 +982,10 @@ int attend(sm_ctx* ctx, const Kv8Attn& args, int head_dim, int B, const char* wh
   Kv8Attn a = args;
   a.status = ctx_status(ctx);
   if (B > 65535 || a.c.n_kv > 65535) return fail(SM_ERR_SHAPE, std::string(what) + ": batch too large");
-  if (!a.prefix.k) {
-    int sms = 0;
-    SM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-    int nl = 0;
-    SM_TRY(launch_decode(a, head_dim, B, device, sms, st, &nl));
+  int sms = 0, nl = 0;
+  SM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  SM_TRY(launch_decode(a, head_dim, B, device, sms, st, &nl));
+  if (nl) {
     *launches += nl;
     return SM_OK;
   }

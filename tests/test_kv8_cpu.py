@@ -15,7 +15,7 @@ def view(k=64, v=64, ks=64, vs=64, seqs=4, tokens=32, n_kv=2, hd=64):
 
 P = 4096  # any non-null address: nothing here is dereferenced
 BAD_CACHES = [
-    (dict(seqs=0), -2), (dict(tokens=0), -2), (dict(n_kv=0), -2), (dict(n_kv=-1), -2),
+    (dict(seqs=0), -2), (dict(tokens=0), -2), (dict(n_kv=0), -2), (dict(n_kv=-1), -2), (dict(n_kv=4097), -5),
     (dict(hd=0), -5), (dict(hd=63), -5), (dict(hd=96), -5), (dict(hd=256), -5),
     (dict(k=None), -1), (dict(v=None), -1), (dict(ks=None), -1), (dict(vs=None), -1),
     (dict(k=72), -1), (dict(v=65), -1), (dict(ks=66), -1), (dict(vs=67), -1),
