@@ -17,82 +17,6 @@
 namespace sm {
 namespace {
 
-struct Kv8Attn {
-  Kv8View c, prefix;  // prefix.k == nullptr: none
-  int prefix_seq, prefix_len;
-  const float* q;
-  int64_t q_stride;
-  const int* seq_ids;
-  const int* lens;
-  int max_len, n_heads;
-  float* out;
-  int* status;
-  bool q_vec;  // rows of q on 16-byte boundaries
-};
-
-constexpr int THREADS = 128;
-
-// One CTA per (query head, sequence): the scores are formed twice, a key a thread.
-template <int HD>
-__global__ void __launch_bounds__(THREADS) attn_kv8_kernel(Kv8Attn a) {
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int g = h / (a.n_heads / a.c.n_kv);
-  const int slot = a.seq_ids ? a.seq_ids[b] : b;
-  if (slot < 0) return;
-  const int len = a.lens[b];
-  if (slot >= a.c.slots || len < 0 || len > a.max_len) {
-    if (threadIdx.x == 0) atomicExch(a.status, SM_ERR_SHAPE);
-    return;
-  }
-  __shared__ float qs[HD], es[THREADS], red[THREADS / 32];
-  const float scale = 1.f / sqrtf((float)HD);
-  for (int d = threadIdx.x; d < HD; d += THREADS) qs[d] = a.q[(int64_t)b * a.q_stride + h * HD + d];
-  __syncthreads();
-  const int total = a.prefix_len + len;
-  auto locate = [&](int j, const Kv8View*& c) {
-    const bool own = j >= a.prefix_len;
-    c = own ? &a.c : &a.prefix;
-    return own ? a.c.at(slot, g, j - a.prefix_len) : a.prefix.at(a.prefix_seq, g, j);
-  };
-  auto score = [&](int j) {
-    const Kv8View* c;
-    const int64_t at = locate(j, c);
-    float s = 0.f;
-    const char4* p = (const char4*)(c->k + at * HD);
-    for (int d = 0; d < HD; d += 4) {
-      const char4 w = p[d / 4];
-      s += qs[d] * w.x + qs[d + 1] * w.y + qs[d + 2] * w.z + qs[d + 3] * w.w;
-    }
-    return s * (c->ks[at] * scale);
-  };
-  float m = -INFINITY;
-  for (int j = threadIdx.x; j < total; j += THREADS) m = fmaxf(m, score(j));
-  m = warp_max(m);
-  if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = m;
-  __syncthreads();
-  for (int w = 0; w < THREADS / 32; ++w) m = fmaxf(m, red[w]);
-  float acc = 0.f, sum = 0.f;
-  for (int j0 = 0; j0 < total; j0 += THREADS) {
-    const int n = min(THREADS, total - j0);
-    __syncthreads();
-    if ((int)threadIdx.x < n) es[threadIdx.x] = kv8_weight(score(j0 + threadIdx.x) - m);
-    __syncthreads();
-    if (threadIdx.x < HD) {  // a tile's own sums first: short chains of roundings
-      float ta = 0.f, ts = 0.f;
-      for (int j = 0; j < n; ++j) {
-        const Kv8View* c;
-        const int64_t at = locate(j0 + j, c);
-        ta += es[j] * ((float)c->v[at * HD + threadIdx.x] * c->vs[at]);
-        ts += es[j];
-      }
-      acc += ta;
-      sum += ts;
-    }
-  }
-  if (threadIdx.x < HD)
-    a.out[((int64_t)b * a.n_heads + h) * HD + threadIdx.x] = total > 0 ? __fdiv_rn(acc, sum) : 0.f;
-}
-
 // ---------------------------------------------------------------- pieces of the decode kernels
 //
 // Keys are taken in blocks of 32, a warp each:
@@ -242,7 +166,7 @@ struct PVSum {
     return T::PA ? (g & 3) * 32 + t * 8 + (g >> 2) * 4 : g * 32 + t * 8;
   }
 
-  float m[T::NT], unit[T::NT], esum[T::NT];  // of this lane's head: factored maximum, factor, sum of weights
+  float m[T::NT], unit[T::NT], esum[T::NT];  // of this lane's head: maximum, factor of the scores, sum of weights
   float mult, back;                          // fixed point: e = 1 at scale vmax is 2^23 - 8
   int acc[T::MD][T::MT][4];
 
@@ -252,7 +176,7 @@ struct PVSum {
     mult = 8388600.f / vmax;
     back = vmax * (1.f / 8388600.f);
 #pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt) unit[nt] = unit_of[nt], m[nt] = max_of[nt] * unit_of[nt], esum[nt] = 0.f;
+    for (int nt = 0; nt < T::NT; ++nt) unit[nt] = unit_of[nt], m[nt] = max_of[nt], esum[nt] = 0.f;
 #pragma unroll
     for (int i = 0; i < T::MD; ++i)
 #pragma unroll
@@ -357,18 +281,6 @@ struct PVSum {
     }
   }
 };
-
-// Row b's slot and length; false where there is nothing to do (padding) or the row is out of range.
-__device__ __forceinline__ bool row_keys(const Kv8Attn& a, int b, int& slot, int& len) {
-  slot = a.seq_ids ? a.seq_ids[b] : b;
-  if (slot < 0) return false;
-  len = a.lens[b];
-  if (slot >= a.c.slots || len < 0 || len > a.max_len) {
-    if (threadIdx.x == 0) atomicExch(a.status, SM_ERR_SHAPE);
-    return false;
-  }
-  return true;
-}
 
 // ---------------------------------------------------------------- a warp's ring
 //
@@ -565,7 +477,7 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) {
     unit[nt] = __shfl_sync(0xffffffffu, unit[nt], col * 4);
-    max_of[nt] = gmax[nt * 8 + col];
+    max_of[nt] = gmax[nt * 8 + col] * unit[nt];
   }
   pv.start(vmax, max_of, unit);
   for (int i = nk; i < nk + nv; ++i) {
@@ -619,15 +531,6 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
 // against the maximum over the chunks; the CTA that finishes a (sequence, kv head) joins its chunks'
 // sums, in order.  The scores add GP * 8 bytes to the 2 * HD + 8 of a key and mostly stay in L2.  Bound by
 // HBM.
-struct Kv8Split {
-  Kv8Attn a;
-  int chunk, n_chunks;  // keys of a chunk (whole blocks); chunks that max_len makes
-  float* z;             // [B][n_kv][NT][blocks] score blocks
-  float* stat;          // [B][n_kv][n_chunks][2 * GP + 1] maxima, largest V scale; then the weights' sums
-  int* arrived;         // [B][n_kv] chunks whose P V is done
-  float* pacc;          // [B][n_kv][n_chunks][GP][HD]
-};
-
 template <int HD, int GP, bool PV>
 struct SplitSmem {
   using S = Slot<HD, GP, PV>;
@@ -726,7 +629,7 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
   if (!row_keys(a, b, slot, len)) return;
   const int j0 = ch * s.chunk, n = min(len - j0, s.chunk);
   if (n <= 0) {
-    if (len == 0 && ch == 0)
+    if (len == 0 && ch == 0 && !s.prefix_max)
       for (int i = tid; i < G * HD; i += DT) a.out[((int64_t)b * a.n_heads + gk * G) * HD + i] = 0.f;
     return;
   }
@@ -783,6 +686,11 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
     max_of[nt] = -INFINITY;
 #pragma unroll
     for (int i = 0; i < DW; ++i) max_of[nt] = fmaxf(max_of[nt], gmax[i][nt * 8 + col]);
+    max_of[nt] *= unit[nt];
+    if (s.prefix_max && nt * 8 + col < G)
+      for (int i = 0; i < s.prefix_chunks; ++i)
+        max_of[nt] = fmaxf(max_of[nt], __ldg(s.prefix_max + ((int64_t)gk * s.prefix_chunks + i) * s.prefix_rows +
+                                             (int64_t)b * G + nt * 8 + col));
   }
   pv.start(vmax, max_of, unit);
   int at = 0;
@@ -825,6 +733,7 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
     for (int i = 0; i < T::TW; ++i) x += wred[i][tid];
     stat[ch * (2 * GP + 1) + GP + 1 + tid] = x;
   }
+  if (s.prefix_max) return;
   // the last CTA of this (sequence, kv head) joins the chunks, always in their order
   __threadfence();
   __syncthreads();
@@ -910,67 +819,64 @@ int launch_decode_cluster(const Kv8Attn& a, int B, const ClusterPlan& plan, cuda
 }
 
 template <int HD, int GP>
-int launch_decode_split(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st) {
-  auto scores = split_scores_kernel<HD, GP>;
-  auto pv = split_pv_kernel<HD, GP>;
-  using SK = SplitSmem<HD, GP, false>;
-  using SV = SplitSmem<HD, GP, true>;
-  static bool ready[64] = {};
-  if (device >= 64) return fail(SM_ERR_UNSUPPORTED, "attention_kv8: device id too large");
-  if (!ready[device]) {
-    SM_CUDA_TRY(cudaFuncSetAttribute(scores, cudaFuncAttributeMaxDynamicSharedMemorySize, SK::RING));
-    SM_CUDA_TRY(cudaFuncSetAttribute(pv, cudaFuncAttributeMaxDynamicSharedMemorySize, SV::RING));
-    ready[device] = true;
-  }
-  Kv8Split s;
-  s.a = a;
-  const int64_t bg = (int64_t)B * a.c.n_kv;
-  // one wave of CTAs where that makes chunks of 512 to 4096 keys (b 1, 131071 keys, 32 / 8 x 128: chunks of
-  // 1024 keys 87 us, of 2048 72 us, one wave of 3552 68 us)
-  const int wave = (int)std::max<int64_t>(1, (int64_t)SV::CTAS * sms / bg);
-  s.chunk = std::min(4096, std::max(512, ((a.max_len + wave - 1) / wave + 31) & ~31));
-  s.n_chunks = (a.max_len + s.chunk - 1) / s.chunk;
-  const int64_t rows = bg * s.n_chunks;
-  const int64_t nz = rows * s.chunk * GP, nstat = rows * (2 * GP + 1), nacc = rows * GP * HD;
-  void* buf = nullptr;
-  if (cudaMallocAsync(&buf, (size_t)(nz + nacc + nstat + bg) * sizeof(float), st) != cudaSuccess) {
-    cudaGetLastError();
-    return fail(SM_ERR_OOM, "attention_kv8: device allocation failed");
-  }
-  s.z = (float*)buf;
-  s.pacc = s.z + nz;
-  s.stat = s.pacc + nacc;
-  s.arrived = (int*)(s.stat + nstat);
+int launch_split(const Kv8Split& s, int B, bool pv, cudaStream_t st) {
+  auto kern = pv ? split_pv_kernel<HD, GP> : split_scores_kernel<HD, GP>;
+  const int smem = pv ? SplitSmem<HD, GP, true>::RING : SplitSmem<HD, GP, false>::RING;
+  SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchAttribute attr[2];
-  const dim3 grid(s.n_chunks, a.c.n_kv, B);
-  cudaLaunchConfig_t cfg = launch_config(grid, DT, SK::RING, st, 1, attr);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, scores, s);
-  cfg.dynamicSmemBytes = SV::RING;
-  if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, pv, s);
-  cudaFreeAsync(buf, st);
-  SM_CUDA_TRY(e);
+  const cudaLaunchConfig_t cfg = launch_config(dim3(s.n_chunks, s.a.c.n_kv, B), DT, smem, st, 1, attr);
+  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, s));
   return SM_OK;
 }
 
+int launch_split_as(const Kv8Split& s, int hd, int B, bool pv, cudaStream_t st) {
+  if (hd == 64)
+    return s.gp == 4   ? launch_split<64, 4>(s, B, pv, st)
+           : s.gp == 8 ? launch_split<64, 8>(s, B, pv, st)
+                       : launch_split<64, 16>(s, B, pv, st);
+  return s.gp == 4   ? launch_split<128, 4>(s, B, pv, st)
+         : s.gp == 8 ? launch_split<128, 8>(s, B, pv, st)
+                     : launch_split<128, 16>(s, B, pv, st);
+}
+
+int launch_decode_split(const Kv8Attn& a, int hd, int B, int sms, cudaStream_t st) {
+  Kv8Split s = {};
+  s.a = a;
+  void* buf = nullptr;
+  if (cudaMallocAsync(&buf, (size_t)kv8_split_plan(s, hd, B, sms) * sizeof(float), st) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(SM_ERR_OOM, "attention_kv8: device allocation failed");
+  }
+  kv8_split_place(s, hd, B, (float*)buf);
+  int rc = launch_split_as(s, hd, B, false, st);
+  if (rc == SM_OK) rc = launch_split_as(s, hd, B, true, st);
+  cudaFreeAsync(buf, st);
+  return rc;
+}
+
+// The cluster form where it applies (plan.size > 0)
 template <int HD, int GP>
-int launch_decode_as(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st, int* n_launch) {
+int try_cluster(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st, int* n_launch) {
   ClusterPlan plan;
   SM_TRY((plan_cluster<HD, GP>(a, B, device, sms, plan)));
-  *n_launch = plan.size ? 1 : a.prefix.k ? 0 : 2;
-  if (plan.size) return launch_decode_cluster<HD, GP>(a, B, plan, st);
-  if (a.prefix.k) return SM_OK;
-  return launch_decode_split<HD, GP>(a, B, device, sms, st);
+  *n_launch = plan.size ? 1 : 0;
+  return plan.size ? launch_decode_cluster<HD, GP>(a, B, plan, st) : SM_OK;
 }
 
 int launch_decode(const Kv8Attn& a, int hd, int B, int device, int sms, cudaStream_t st, int* n_launch) {
   const int G = a.n_heads / a.c.n_kv;
   if (hd == 64)
-    return G <= 4   ? launch_decode_as<64, 4>(a, B, device, sms, st, n_launch)
-           : G <= 8 ? launch_decode_as<64, 8>(a, B, device, sms, st, n_launch)
-                    : launch_decode_as<64, 16>(a, B, device, sms, st, n_launch);
-  return G <= 4   ? launch_decode_as<128, 4>(a, B, device, sms, st, n_launch)
-         : G <= 8 ? launch_decode_as<128, 8>(a, B, device, sms, st, n_launch)
-                  : launch_decode_as<128, 16>(a, B, device, sms, st, n_launch);
+    SM_TRY(G <= 4   ? (try_cluster<64, 4>(a, B, device, sms, st, n_launch))
+           : G <= 8 ? (try_cluster<64, 8>(a, B, device, sms, st, n_launch))
+                    : (try_cluster<64, 16>(a, B, device, sms, st, n_launch)));
+  else
+    SM_TRY(G <= 4   ? (try_cluster<128, 4>(a, B, device, sms, st, n_launch))
+           : G <= 8 ? (try_cluster<128, 8>(a, B, device, sms, st, n_launch))
+                    : (try_cluster<128, 16>(a, B, device, sms, st, n_launch)));
+  if (*n_launch) return SM_OK;
+  if (a.prefix_len > 0) return launch_attention_shared_tc(a, hd, B, sms, st, n_launch);
+  *n_launch = 2;
+  return launch_decode_split(a, hd, B, sms, st);
 }
 
 int attend(sm_ctx* ctx, const Kv8Attn& args, int head_dim, int B, const char* what) {
@@ -985,17 +891,7 @@ int attend(sm_ctx* ctx, const Kv8Attn& args, int head_dim, int B, const char* wh
   int sms = 0, nl = 0;
   SM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
   SM_TRY(launch_decode(a, head_dim, B, device, sms, st, &nl));
-  if (nl) {
-    *launches += nl;
-    return SM_OK;
-  }
-  const dim3 grid(a.n_heads, B);
-  if (head_dim == 64)
-    attn_kv8_kernel<64><<<grid, THREADS, 0, st>>>(a);
-  else
-    attn_kv8_kernel<128><<<grid, THREADS, 0, st>>>(a);
-  SM_CUDA_TRY(cudaGetLastError());
-  *launches += 1;
+  *launches += nl;
   return SM_OK;
 }
 
@@ -1016,6 +912,37 @@ int check_attn(sm_ctx* ctx, const sm_kv8* c, const float* q, int64_t q_stride, c
 }
 
 }  // namespace
+
+int64_t kv8_split_plan(Kv8Split& s, int hd, int B, int sms) {
+  const int G = s.a.n_heads / s.a.c.n_kv;
+  s.gp = G <= 4 ? 4 : G <= 8 ? 8 : 16;
+  const int64_t bg = (int64_t)B * s.a.c.n_kv;
+  // one wave of CTAs (2 an SM, or 1 where a group's accumulators fill the registers) where that makes chunks of
+  // 512 to 4096 keys (b 1, 131071 keys, 32 / 8 x 128: chunks of 1024 keys 87 us, of 2048 72 us, one wave of
+  // 3552 68 us)
+  const int ctas = s.gp == 4 || (hd == 64 && s.gp == 8) ? 2 : 1;
+  const int64_t wave = std::max<int64_t>(1, (int64_t)ctas * sms / bg);
+  s.chunk = (int)std::min<int64_t>(4096, std::max<int64_t>(512, ((s.a.max_len + wave - 1) / wave + 31) & ~31LL));
+  s.n_chunks = ceil_div(s.a.max_len, s.chunk);
+  const int64_t rows = bg * s.n_chunks;
+  return rows * s.chunk * s.gp + rows * s.gp * hd + rows * (2 * s.gp + 1) + bg;
+}
+
+void kv8_split_place(Kv8Split& s, int hd, int B, float* base) {
+  const int64_t bg = (int64_t)B * s.a.c.n_kv, rows = bg * s.n_chunks;
+  s.z = base;
+  s.pacc = s.z + rows * s.chunk * s.gp;
+  s.stat = s.pacc + rows * s.gp * hd;
+  s.arrived = (int*)(s.stat + rows * (2 * s.gp + 1));
+}
+
+int launch_kv8_split_scores(const Kv8Split& s, int hd, int B, cudaStream_t st) {
+  return launch_split_as(s, hd, B, false, st);
+}
+int launch_kv8_split_pv(const Kv8Split& s, int hd, int B, cudaStream_t st) {
+  return launch_split_as(s, hd, B, true, st);
+}
+
 }  // namespace sm
 
 using namespace sm;

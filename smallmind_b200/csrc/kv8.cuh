@@ -44,4 +44,54 @@ inline cudaLaunchConfig_t launch_config(dim3 grid, int threads, size_t smem, cud
   return cfg;
 }
 
+// One decode attention call.
+struct Kv8Attn {
+  Kv8View c, prefix;  // prefix.k == nullptr: none
+  int prefix_seq, prefix_len;
+  const float* q;
+  int64_t q_stride;
+  const int* seq_ids;
+  const int* lens;
+  int max_len, n_heads;
+  float* out;
+  int* status;
+  bool q_vec;  // rows of q on 16-byte boundaries
+};
+
+// Row b's slot and length; false where there is nothing to do (padding) or the row is out of range.
+__device__ __forceinline__ bool row_keys(const Kv8Attn& a, int b, int& slot, int& len) {
+  slot = a.seq_ids ? a.seq_ids[b] : b;
+  if (slot < 0) return false;
+  len = a.lens[b];
+  if (slot >= a.c.slots || len < 0 || len > a.max_len) {
+    if (threadIdx.x == 0) atomicExch(a.status, SM_ERR_SHAPE);
+    return false;
+  }
+  return true;
+}
+
+// The long form of the decode attention (attn_kv8.cu): scores of chunks of keys, then P V.  Also the own keys
+// of the batch behind a shared prefix, whose maxima and sums then come from attn_kv8_tc.cu.
+struct Kv8Split {
+  Kv8Attn a;
+  int chunk, n_chunks;  // keys of a chunk (whole blocks of 32); chunks that max_len makes
+  int gp;               // heads a kv head's group is padded to: 4, 8 or 16
+  float* z;             // [B][n_kv][gp / 8 or 1][blocks] blocks of scores
+  float* pacc;          // [B][n_kv][n_chunks][gp][head_dim]
+  float* stat;          // [B][n_kv][n_chunks][2 * gp + 1] maxima, largest V scale; then the weights' sums
+  int* arrived;         // [B][n_kv] chunks whose P V is done
+  // behind a shared prefix: its scores' maxima [n_kv][prefix_chunks][prefix_rows], row b * group + head, as
+  // z = (q . k) / sqrt(head_dim); the chunks are then joined by the caller
+  const float* prefix_max;
+  int prefix_chunks, prefix_rows;
+};
+// Sizes chunk, n_chunks and gp; returns the floats that z, pacc, stat and arrived take together.
+int64_t kv8_split_plan(Kv8Split& s, int head_dim, int B, int sms);
+void kv8_split_place(Kv8Split& s, int head_dim, int B, float* base);
+int launch_kv8_split_scores(const Kv8Split& s, int head_dim, int B, cudaStream_t st);
+int launch_kv8_split_pv(const Kv8Split& s, int head_dim, int B, cudaStream_t st);
+
+// attn_kv8_tc.cu: decode attention behind a shared prefix (prefix_len > 0) on tcgen05
+int launch_attention_shared_tc(const Kv8Attn& a, int head_dim, int B, int sms, cudaStream_t st, int* n_launch);
+
 }  // namespace sm

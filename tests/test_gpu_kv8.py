@@ -366,6 +366,60 @@ def test_shared_prefix(ctx, n_heads, n_kv, hd, B, prefix_len):
         assert not got[0].any()
 
 
+@pytest.mark.parametrize("n_heads,n_kv,hd,B,prefix_len,longest", [
+    (32, 4, 64, 64, 3001, 90), (9, 3, 64, 90, 2705, 33), (8, 8, 64, 40, 2688, 0), (32, 8, 128, 17, 3100, 700),
+    (16, 1, 128, 130, 2817, 40), (7, 1, 64, 260, 6500, 5), (12, 4, 128, 150, 1500, 1), (2, 2, 128, 300, 700, 64)])
+def test_long_shared_prefix(ctx, n_heads, n_kv, hd, B, prefix_len, longest):
+    """Batches times prefixes beyond what a cluster per row reads: the matrix form."""
+    rs = np.random.RandomState(B + prefix_len)
+    lens = rs.randint(0, longest + 1, B)
+    lens[0], lens[-1] = 0, longest
+    seq = rs.permutation(B + 2)[:B]
+    seq[B // 2] = -1
+    held = np.zeros(B + 2, int)
+    held[seq[seq >= 0]] = lens[seq >= 0]
+    p = Cache(ctx, 1, prefix_len, n_kv, hd).fill(rs, [prefix_len])
+    c = Cache(ctx, B + 2, max(1, longest), n_kv, hd).fill(rs, held)
+    q = (rs.randn(B, n_heads, hd) * np.exp(rs.randn(B, n_heads, 1))).astype(np.float32)
+    q[1, 0] = 0
+    a, pa = c.arrays(), p.arrays()
+    keys = [None if s < 0 else [(pa, 0, prefix_len), (a, s, n)] for s, n in zip(seq, lens)]
+    want, tol = kv8_ref.attend_rows(q, n_kv, keys)
+    got = run_decode(ctx, c, q, seq, lens, longest, prefix=p, prefix_len=prefix_len, q_stride=n_heads * hd + 1)
+    check(got, want, tol)
+    assert (got[B // 2] == 5.0).all()
+    assert np.array_equal(got, run_decode(ctx, c, q, seq, lens, longest, prefix=p, prefix_len=prefix_len))
+    assert ctx.device_status() == 0
+
+
+def test_long_shared_prefix_nan_and_bad_rows():
+    """NaNs of q and of the scales reach what depends on them, bad rows set the status, in the matrix form too."""
+    import smallmind_b200 as sm
+    ctx = sm.CudaContext(0)
+    rs = np.random.RandomState(77)
+    n_heads, n_kv, hd, B, P = 32, 4, 64, 70, 2900
+    lens = np.full(B, 9)
+    p = Cache(ctx, 1, P + 40, n_kv, hd).fill(rs, [P])
+    c = Cache(ctx, B, 9, n_kv, hd).fill(rs, lens)
+    q = rs.randn(B, n_heads, hd).astype(np.float32)
+    q[3, 9, 5], q[4, 1, 0] = np.nan, np.inf
+    seq = np.arange(B)
+    seq[5], seq[6] = B, -1
+    lens[7], lens[8] = 10, -1
+    p.ks[0, 3, P - 1] = float("nan")
+    c.vs[10, 0, 8] = float("nan")
+    got = run_decode(ctx, c, q, seq, lens, 9, prefix=p, prefix_len=P)
+    assert (got[[5, 6, 7, 8]] == 5.0).all()
+    nan = np.isnan(got).all(-1)
+    assert np.array_equal(nan, np.isnan(got).any(-1))
+    want = np.zeros((B, n_heads), bool)
+    want[:, 24:], want[3, 9], want[4, 1], want[10, :8] = True, True, True, True
+    want[[5, 6, 7, 8]] = False
+    assert np.array_equal(nan, want)
+    assert ctx.device_status() == -2
+    ctx.close()
+
+
 def test_shared_equals_decode_over_a_copied_prefix(ctx):
     """The shared form against the plain decode call over slots that hold the prefix and the own keys in a row."""
     import torch
