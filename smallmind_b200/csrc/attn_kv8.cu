@@ -67,10 +67,10 @@ __device__ __forceinline__ void load_q(const float* q, bool vec, int G, int lane
     if (vec) {
 #pragma unroll
       for (int i = 0; i < HD / 4; i += 4)
-        *(float4*)(x + i) = h < G ? __ldg((const float4*)(q + h * HD + (i / 16) * 64 + 16 * t + i % 16)) : float4{};
+        *(float4*)(x + i) = h < G ? *(const float4*)(q + h * HD + (i / 16) * 64 + 16 * t + i % 16) : float4{};
     } else {
 #pragma unroll
-      for (int i = 0; i < HD / 4; ++i) x[i] = h < G ? __ldg(q + h * HD + (i / 16) * 64 + 16 * t + i % 16) : 0.f;
+      for (int i = 0; i < HD / 4; ++i) x[i] = h < G ? q[h * HD + (i / 16) * 64 + 16 * t + i % 16] : 0.f;
     }
 #pragma unroll
     for (int i = 0; i < HD / 4; ++i) peak = max_nan(peak, fabsf(x[i]));
@@ -624,11 +624,16 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float wred[DW][GP], gmax[DW][GP];
   __shared__ bool last;
-  // everything but the scores and maxima was there before the first kernel let this one start
+  // everything but the scores and maxima was there before the first kernel let this one start; a CTA without work
+  // waits too, or the grid could end before the one it depends on
   int slot, len;
-  if (!row_keys(a, b, slot, len)) return;
+  if (!row_keys(a, b, slot, len)) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   const int j0 = ch * s.chunk, n = min(len - j0, s.chunk);
   if (n <= 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (len == 0 && ch == 0 && !s.prefix_max)
       for (int i = tid; i < G * HD; i += DT) a.out[((int64_t)b * a.n_heads + gk * G) * HD + i] = 0.f;
     return;
@@ -687,10 +692,10 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
 #pragma unroll
     for (int i = 0; i < DW; ++i) max_of[nt] = fmaxf(max_of[nt], gmax[i][nt * 8 + col]);
     max_of[nt] *= unit[nt];
-    if (s.prefix_max && nt * 8 + col < G)
-      for (int i = 0; i < s.prefix_chunks; ++i)
-        max_of[nt] = fmaxf(max_of[nt], __ldg(s.prefix_max + ((int64_t)gk * s.prefix_chunks + i) * s.prefix_rows +
-                                             (int64_t)b * G + nt * 8 + col));
+    if (s.prefix_max && nt * 8 + col < G) {
+      const int64_t row = (int64_t)gk * s.prefix_rows + (int64_t)b * G + nt * 8 + col;
+      max_of[nt] = fmaxf(max_of[nt], s.prefix_max[row] * s.prefix_unit[row]);
+    }
   }
   pv.start(vmax, max_of, unit);
   int at = 0;

@@ -34,6 +34,9 @@ namespace {
 
 constexpr int THREADS = 256;
 
+// The kernels are launched before the one ahead of them on the stream has ended and wait for it themselves, so
+// what they read may still be written while they run: no __restrict__, no read-only loads.
+
 // Whether a row is neither padding nor out of range
 __device__ __forceinline__ bool in_cache(const Kv8View& c, int slot, int pos, int* status) {
   if (slot < 0) return false;
@@ -93,16 +96,16 @@ struct Share {
 };
 
 template <int HD, int N, bool VEC>
-__global__ void __launch_bounds__(THREADS) kv8_write_kernel(Kv8View c, const float* __restrict__ k,
-                                                            const float* __restrict__ v, int64_t row_stride,
-                                                            const int* __restrict__ seq_ids,
-                                                            const int* __restrict__ positions, int n_rows,
+__global__ void __launch_bounds__(THREADS) kv8_write_kernel(Kv8View c, const float* k,
+                                                            const float* v, int64_t row_stride,
+                                                            const int* seq_ids,
+                                                            const int* positions, int n_rows,
                                                             int* status) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Share<HD, N> w(c);
   if (w.row >= n_rows) return;
-  const int slot = __ldg(seq_ids + w.row), pos = __ldg(positions + w.row);
+  const int slot = seq_ids[w.row], pos = positions[w.row];
   const float* src = (w.is_v ? v : k) + w.row * row_stride + w.value;
   float x[N][4];
 #pragma unroll
@@ -145,16 +148,16 @@ __global__ void __launch_bounds__(THREADS) kv8_write_kernel(Kv8View c, const flo
 }
 
 template <int HD, int N, bool VEC>
-__global__ void __launch_bounds__(THREADS) kv8_read_kernel(Kv8View c, const int* __restrict__ seq_ids,
-                                                           const int* __restrict__ positions, int n_rows,
-                                                           float* __restrict__ k, float* __restrict__ v,
+__global__ void __launch_bounds__(THREADS) kv8_read_kernel(Kv8View c, const int* seq_ids,
+                                                           const int* positions, int n_rows,
+                                                           float* k, float* v,
                                                            int64_t row_stride, int* status) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Share<HD, N> w(c);
   float* to = w.is_v ? v : k;
   if (w.row >= n_rows || !to) return;
-  const int slot = __ldg(seq_ids + w.row), pos = __ldg(positions + w.row);
+  const int slot = seq_ids[w.row], pos = positions[w.row];
   if (!in_cache(c, slot, pos, status)) return;
   const int64_t at = w.at(c, slot, pos);
   const int8_t* codes = (w.is_v ? c.v : c.k) + at * HD + w.dim;

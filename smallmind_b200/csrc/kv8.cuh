@@ -25,7 +25,9 @@ inline Kv8View kv8_view(const sm_kv8* c) {
 }
 
 // Launch on a stream after its previous kernel by programmatic dependent launch: the kernel waits
-// (griddepcontrol.wait) before it touches memory.  attr backs the result.
+// (griddepcontrol.wait) before it touches memory.  What it reads may thus be written while it already runs, so
+// none of it goes through __restrict__ or the read-only path, whose loads may move ahead of the wait.  attr
+// backs the result.
 inline cudaLaunchConfig_t launch_config(dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster,
                                  cudaLaunchAttribute (&attr)[2]) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -80,10 +82,11 @@ struct Kv8Split {
   float* pacc;          // [B][n_kv][n_chunks][gp][head_dim]
   float* stat;          // [B][n_kv][n_chunks][2 * gp + 1] maxima, largest V scale; then the weights' sums
   int* arrived;         // [B][n_kv] chunks whose P V is done
-  // behind a shared prefix: its scores' maxima [n_kv][prefix_chunks][prefix_rows], row b * group + head, as
-  // z = (q . k) / sqrt(head_dim); the chunks are then joined by the caller
+  // behind a shared prefix: the largest raw score of row b * group + head, [n_kv][prefix_rows], and its factor
+  // (z = score * unit); the chunks are then joined by the caller
   const float* prefix_max;
-  int prefix_chunks, prefix_rows;
+  const float* prefix_unit;
+  int prefix_rows;
 };
 // Sizes chunk, n_chunks and gp; returns the floats that z, pacc, stat and arrived take together.
 int64_t kv8_split_plan(Kv8Split& s, int head_dim, int B, int sms);

@@ -78,6 +78,42 @@ __device__ __forceinline__ float kv8_weight(float x) {
   return fmaf(6.f, c, a) * r;
 }
 
+// Two floats in one register pair, and their arithmetic in one instruction
+struct Pair {
+  uint64_t v;
+  __device__ __forceinline__ Pair() {}
+  __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ explicit Pair(float a) : Pair(a, a) {}
+  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// kv8_weight of two values
+__device__ __forceinline__ Pair kv8_weight2(Pair x) {
+  float a, b;
+  x.get(a, b);
+  const Pair c(max_nan(a, -87.3f), max_nan(b, -87.3f));
+  const Pair s = fma2(c, c, Pair(12.f));
+  fma2(c, Pair(-6.f), s).get(a, b);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+  return mul2(fma2(c, Pair(6.f), s), Pair(a, b));
+}
+
 // Asynchronous copies into shared memory, in groups that a warp waits for itself
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
