@@ -82,17 +82,27 @@ __device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr) {
 __host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
   return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
+// One lane of a converged warp.  The MMA warp runs as a whole and only the instructions themselves are left to
+// one lane: their operands then stay in uniform registers (issued from a one-lane branch, an MMA took 66 to 80
+// clocks to issue, which bound both passes).
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
 // A from TMEM: lane = row, a 32-bit column holds two neighbouring k
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(acc)
-      : "memory");
+  if (elect())
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"(acc)
+        : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+  if (elect())
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -300,7 +310,7 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
   uint64_t* v_free = v_full + M::NV;
   uint32_t* tmem_slot = (uint32_t*)(v_free + M::NV);
   const Kv8Attn& a = s.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const int cta = blockIdx.x, units = a.c.n_kv * s.tiles * s.n_blocks;
   const int u0 = cta * s.per, u1 = min(units, u0 + s.per);
 
@@ -323,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp == LOAD_WARP) {
     if (lane == 0) {
@@ -352,58 +362,60 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
       }
     }
   } else if (warp == MMA_WARP) {
-    if (lane == 0) {
-      const uint32_t ka = smem_u32(smem + M::K), va = smem_u32(smem + M::V);
-      bool ok = true;
-      Ring k, v, sb, pb;  // K and V slots; score buffers of the next scores and of the next P V
-      int formed = 0;     // blocks whose scores have been started
-      auto scores = [&]() {
-        ok = ok && mbar_wait_bounded(&k_full[k.slot], k.parity, a.status);
-        if (formed >= M::NS)
-          ok = ok && mbar_wait_bounded(MAX ? &s_done[sb.slot] : &pv_done[sb.slot], sb.parity ^ 1, a.status);
-        if (!ok) return;
-        tc_fence_after();
+    const uint64_t kd0 = sw128_desc(smem_u32(smem + M::K)), vd0 = sw128_desc_mn(smem_u32(smem + M::V));
+    bool ok = true;
+    auto wait = [&](uint64_t* b, int parity) {
+      ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(b, parity, a.status));
+    };
+    Ring k, v, sb, pb;  // K and V slots; score buffers of the next scores and of the next P V
+    int formed = 0;     // blocks whose scores have been started
+    auto scores = [&]() {
+      wait(&k_full[k.slot], k.parity);
+      if (formed >= M::NS) wait(MAX ? &s_done[sb.slot] : &pv_done[sb.slot], sb.parity ^ 1);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t kd = kd0 + (uint32_t)(k.slot * (M::TILE >> 4));
+      const uint32_t sd = tmem + TM_S + sb.slot * KB;
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-          const uint64_t kd = sw128_desc(ka + k.slot * M::TILE + (uint32_t)((i >> 2) * (KB * 128) + (i & 3) * 32));
-          mma_ts(tmem + TM_S + sb.slot * KB, tmem + TM_Q + 8 * i, kd, idesc(KB, false), i != 0);
-          mma_ts(tmem + TM_S + sb.slot * KB, tmem + TM_Q + HD / 2 + 8 * i, kd, idesc(KB, false), 1);
-        }
-        mma_commit(&s_full[sb.slot]);
-        mma_commit(&k_free[k.slot]);
-        k.next<M::NK>();
-        sb.next<M::NS>();
-        ++formed;
-      };
-      int seg = 0;
-      for (int u = u0; u < u1 && ok; ++seg) {
-        const int nb = min(u1 - u, s.n_blocks - u % s.n_blocks);
-        ok = mbar_wait_bounded(q_full, seg & 1, a.status);
-        tc_fence_after();
-        for (int i = 0; i < min(nb, M::NS) && ok; ++i) scores();
-        for (int i = 0; i < nb && ok; ++i) {
-          if constexpr (!MAX) {
-            ok = mbar_wait_bounded(&v_full[v.slot], v.parity, a.status) &&
-                 mbar_wait_bounded(&s_done[pb.slot], pb.parity, a.status);
-            if (!ok) break;
-            tc_fence_after();
-#pragma unroll
-            for (int j = 0; j < KB / 16; ++j) {
-              // keys 16 j ..: P hi, then lo, in the score columns of these keys
-              const uint32_t p = tmem + TM_S + pb.slot * KB + 16 * j;
-              const uint64_t vd = sw128_desc_mn(va + v.slot * M::TILE + (uint32_t)j * (16 * 128));
-              mma_ts(tmem + TM_O, p, vd, idesc(HD, true), i % FLUSH | j ? 1 : 0);
-              mma_ts(tmem + TM_O, p + 8, vd, idesc(HD, true), 1);
-            }
-            mma_commit(&pv_done[pb.slot]);
-            mma_commit(&v_free[v.slot]);
-            v.next<M::NV>();
-            pb.next<M::NS>();
-          }
-          if (i + M::NS < nb) scores();
-        }
-        u += nb;
+      for (int i = 0; i < HD / 16; ++i) {
+        const uint64_t d = kd + (uint32_t)(((i >> 2) * (KB * 128) + (i & 3) * 32) >> 4);
+        mma_ts(sd, tmem + TM_Q + 8 * i, d, idesc(KB, false), i != 0);
+        mma_ts(sd, tmem + TM_Q + HD / 2 + 8 * i, d, idesc(KB, false), 1);
       }
+      mma_commit(&s_full[sb.slot]);
+      mma_commit(&k_free[k.slot]);
+      k.next<M::NK>();
+      sb.next<M::NS>();
+      ++formed;
+    };
+    int seg = 0;
+    for (int u = u0; u < u1 && ok; ++seg) {
+      const int nb = min(u1 - u, s.n_blocks - u % s.n_blocks);
+      wait(q_full, seg & 1);
+      tc_fence_after();
+      for (int i = 0; i < min(nb, M::NS) && ok; ++i) scores();
+      for (int i = 0; i < nb && ok; ++i) {
+        if constexpr (!MAX) {
+          wait(&v_full[v.slot], v.parity);
+          wait(&s_done[pb.slot], pb.parity);
+          if (!ok) break;
+          tc_fence_after();
+          // keys 16 j ..: P hi, then lo, in the score columns of these keys
+          const uint32_t p = tmem + TM_S + pb.slot * KB;
+          const uint64_t vd = vd0 + (uint32_t)(v.slot * (M::TILE >> 4));
+#pragma unroll
+          for (int j = 0; j < KB / 16; ++j) {
+            mma_ts(tmem + TM_O, p + 16 * j, vd + j * (16 * 128 >> 4), idesc(HD, true), i % FLUSH | j ? 1 : 0);
+            mma_ts(tmem + TM_O, p + 16 * j + 8, vd + j * (16 * 128 >> 4), idesc(HD, true), 1);
+          }
+          mma_commit(&pv_done[pb.slot]);
+          mma_commit(&v_free[v.slot]);
+          v.next<M::NV>();
+          pb.next<M::NS>();
+        }
+        if (i + M::NS < nb) scores();
+      }
+      u += nb;
     }
   } else {
     const int r = (warp & 3) * 32 + lane, part = warp >> 2;
