@@ -9,6 +9,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include "kv8.cuh"
 #include "kv8_mma.cuh"
@@ -21,9 +22,9 @@ namespace {
 //
 // Keys are taken in blocks of 32, a warp each:
 //   scores  two 16-key x 8-head MMA tiles.  K codes are A fragments as they lie: a lane takes 16
-//           neighbouring bytes of a row, and q's digits, built once, are in the matching order.  A lane's four rows are the keys whose scores the P side wants
-//           side by side.  Scores are kept without the head's positive factor, which a maximum
-//           does not need;
+//           neighbouring bytes of a row, and q's digits, built once, are in the matching order.  A lane's
+//           four rows are the keys whose scores the P side wants side by side.  Scores are kept without the
+//           head's positive factor, which a maximum does not need;
 //   P V     weights e, and P = e * v_scale in 23-bit fixed point against the largest v_scale of
 //           the warp's keys, in the registers that the MMA wants them in; V codes are made
 //           fragments by 4 x 4 byte transposes.  With up to 4 heads the three digits of all of
@@ -365,10 +366,11 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 
 // ---------------------------------------------------------------- decode, short: one cluster per (sequence, kv head)
 //
-// One launch: the keys (a shared prefix's blocks first, then the sequence's own) are split over the cluster's CTAs, the scores stay in shared memory, and the
-// exact maximum and the sums travel through distributed shared memory.  A warp's K blocks and then its
-// V blocks go through one ring, so V is on its way while the maxima are exchanged.  Bound by its chain of
-// phases.
+// One launch: the keys (a shared prefix's blocks first, then the sequence's own) are split over the cluster's
+// CTAs, the scores stay in shared memory, and the exact maximum and the sums travel through distributed shared
+// memory.  Behind a prefix (o) the weights are formed against the larger of both maxima and the sums are left to
+// be joined.  A warp's K blocks and then its V blocks go through one ring, so V is on its way while the maxima
+// are exchanged.  Bound by its chain of phases.
 template <int HD, int GP>
 struct ClusterSmem {
   using T = Tile<HD, GP>;
@@ -381,7 +383,8 @@ struct ClusterSmem {
 };
 
 template <int HD, int GP>
-__global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1) decode_kv8_kernel(Kv8Attn a, int cap) {
+__global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1)
+    decode_kv8_kernel(Kv8Attn a, Kv8Behind o, int cap) {
   using T = Tile<HD, GP>;
   using M = ClusterSmem<HD, GP>;
   using S = Slot<HD, GP, false>;
@@ -401,9 +404,12 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   int slot, len;
   if (!row_keys(a, b, slot, len)) return;
   float* out = a.out + ((int64_t)b * a.n_heads + gk * G) * HD;
+  const int64_t row0 = (int64_t)gk * o.rows + (int64_t)b * G;  // behind a prefix
   if (a.prefix_len + len == 0) {
-    if (rank == 0)
-      for (int i = tid; i < G * HD; i += DT) out[i] = 0.f;
+    if (rank == 0) {
+      for (int i = tid; i < G * HD; i += DT) (o.prefix_max ? o.acc + row0 * HD : out)[i] = 0.f;
+      if (o.prefix_max && tid < G) o.sum[row0 + tid] = 0.f;
+    }
     return;
   }
   // this CTA's blocks of all: the prefix's np, then the sequence's own
@@ -429,8 +435,8 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
       const int blk = b0 + (is_k ? warp + DW * i : tw + T::TW * (i - nk));
       const bool shared = blk < np;
       const Kv8View& c = shared ? a.prefix : a.c;
-      const int64_t row0 = shared ? prefix0 : own0;
-      S::fetch(ring_at + i % M::N * S::BYTES, (is_k ? c.k : c.v) + row0 * HD, is_k ? c.ks + row0 : nullptr, c.vs + row0,
+      const int64_t at = shared ? prefix0 : own0;
+      S::fetch(ring_at + i % M::N * S::BYTES, (is_k ? c.k : c.v) + at * HD, is_k ? c.ks + at : nullptr, c.vs + at,
                32 * (shared ? blk : blk - np), shared ? a.prefix_len : len, lane, shared ? often : once);
     }
     cp_commit();
@@ -478,6 +484,11 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   for (int nt = 0; nt < T::NT; ++nt) {
     unit[nt] = __shfl_sync(0xffffffffu, unit[nt], col * 4);
     max_of[nt] = gmax[nt * 8 + col] * unit[nt];
+    const int h = nt * 8 + col;
+    if (o.prefix_max && h < G) {
+      if (rank == 0 && warp == 0 && t == 0 && g == col) o.own_max[row0 + h] = max_of[nt];
+      max_of[nt] = fmaxf(max_of[nt], o.prefix_max[row0 + h] * o.prefix_unit[row0 + h]);
+    }
   }
   pv.start(vmax, max_of, unit);
   for (int i = nk; i < nk + nv; ++i) {
@@ -519,7 +530,12 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
       s += cluster.map_shared_rank(pacc, r)[i];
       total += cluster.map_shared_rank(stat, r)[GP + i / HD];
     }
-    out[i] = __fdiv_rn(s, total);
+    if (o.prefix_max) {
+      o.acc[row0 * HD + i] = s;
+      if (i % HD == 0) o.sum[row0 + i / HD] = total;
+    } else {
+      out[i] = __fdiv_rn(s, total);
+    }
   }
   cluster.sync();  // no CTA's shared memory goes before the others have read it
 }
@@ -531,6 +547,17 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
 // against the maximum over the chunks; the CTA that finishes a (sequence, kv head) joins its chunks'
 // sums, in order.  The scores add GP * 8 bytes to the 2 * HD + 8 of a key and mostly stay in L2.  Bound by
 // HBM.
+struct Kv8Split {
+  Kv8Attn a;
+  Kv8Behind o;
+  int chunk, n_chunks;  // keys of a chunk (whole blocks); chunks that max_len makes
+  int gp;               // heads a kv head's group is padded to: 4, 8 or 16
+  float* z;             // [B][n_kv][gp / 8 or 1][blocks] blocks of scores
+  float* pacc;          // [B][n_kv][n_chunks][gp][head_dim]
+  float* stat;          // [B][n_kv][n_chunks][2 * gp + 1] maxima, largest V scale; then the weights' sums
+  int* arrived;         // [B][n_kv] chunks whose P V is done
+};
+
 template <int HD, int GP, bool PV>
 struct SplitSmem {
   using S = Slot<HD, GP, PV>;
@@ -552,7 +579,7 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, false>::CTAS)) split_sc
   const int G = a.n_heads / a.c.n_kv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float wred[DW][GP], vred[DW];
+  __shared__ float wred[DW][GP], vred[DW], unit_of[GP];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // only now: what the next kernel reads before its own wait has then been written
   asm volatile("griddepcontrol.launch_dependents;");
@@ -598,6 +625,11 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, false>::CTAS)) split_sc
   warp_maxima<HD, GP>(mx, g, t, wred[warp]);
   vmax = warp_max_nan(vmax);
   if (lane == 0) vred[warp] = vmax;
+  if (warp == 0 && t == 0) {
+#pragma unroll
+    for (int nt = 0; nt < T::NT; ++nt)
+      if (g < T::CP) unit_of[nt * 8 + g] = unit[nt];
+  }
   __syncthreads();
   float* stat = s.stat + (bg * s.n_chunks + ch) * (2 * GP + 1);
   if (tid < GP) {
@@ -605,6 +637,8 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, false>::CTAS)) split_sc
 #pragma unroll
     for (int i = 0; i < DW; ++i) m = fmaxf(m, wred[i][tid]);
     stat[tid] = m;
+    if (s.o.prefix_max && tid < G)
+      atomic_max(s.o.own_max + (int64_t)gk * s.o.rows + (int64_t)b * G + tid, m * unit_of[tid]);
   } else if (tid == GP) {
 #pragma unroll
     for (int i = 0; i < DW; ++i) vmax = max_nan(vmax, vred[i]);
@@ -632,15 +666,19 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
     return;
   }
   const int j0 = ch * s.chunk, n = min(len - j0, s.chunk);
+  const int64_t row0 = (int64_t)gk * s.o.rows + (int64_t)b * G;  // behind a prefix
   if (n <= 0) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (len == 0 && ch == 0 && !s.prefix_max)
-      for (int i = tid; i < G * HD; i += DT) a.out[((int64_t)b * a.n_heads + gk * G) * HD + i] = 0.f;
+    if (len == 0 && ch == 0) {
+      float* to = s.o.prefix_max ? s.o.acc + row0 * HD : a.out + ((int64_t)b * a.n_heads + gk * G) * HD;
+      for (int i = tid; i < G * HD; i += DT) to[i] = 0.f;
+      if (s.o.prefix_max && tid < G) s.o.sum[row0 + tid] = 0.f;
+    }
     return;
   }
-  const int64_t row0 = a.c.at(slot, gk, j0);
-  const int8_t* vp = a.c.v + row0 * HD;
-  const float* vsp = a.c.vs + row0;
+  const int64_t first = a.c.at(slot, gk, j0);
+  const int8_t* vp = a.c.v + first * HD;
+  const float* vsp = a.c.vs + first;
   const int64_t bg = (int64_t)b * a.c.n_kv + gk;
   const int64_t plane = (int64_t)s.n_chunks * s.chunk * T::CP;
   const int tw = warp / T::DS, d0 = (warp % T::DS) * T::DP;
@@ -692,9 +730,9 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
 #pragma unroll
     for (int i = 0; i < DW; ++i) max_of[nt] = fmaxf(max_of[nt], gmax[i][nt * 8 + col]);
     max_of[nt] *= unit[nt];
-    if (s.prefix_max && nt * 8 + col < G) {
-      const int64_t row = (int64_t)gk * s.prefix_rows + (int64_t)b * G + nt * 8 + col;
-      max_of[nt] = fmaxf(max_of[nt], s.prefix_max[row] * s.prefix_unit[row]);
+    if (s.o.prefix_max && nt * 8 + col < G) {
+      const int64_t row = row0 + nt * 8 + col;
+      max_of[nt] = fmaxf(max_of[nt], s.o.prefix_max[row] * s.o.prefix_unit[row]);
     }
   }
   pv.start(vmax, max_of, unit);
@@ -738,7 +776,6 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
     for (int i = 0; i < T::TW; ++i) x += wred[i][tid];
     stat[ch * (2 * GP + 1) + GP + 1 + tid] = x;
   }
-  if (s.prefix_max) return;
   // the last CTA of this (sequence, kv head) joins the chunks, always in their order
   __threadfence();
   __syncthreads();
@@ -753,7 +790,12 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
       x += __ldcg(s.pacc + (bg * s.n_chunks + c) * GP * HD + i);
       total += __ldcg(stat + c * (2 * GP + 1) + GP + 1 + i / HD);
     }
-    a.out[((int64_t)b * a.n_heads + gk * G) * HD + i] = __fdiv_rn(x, total);
+    if (s.o.prefix_max) {
+      s.o.acc[row0 * HD + i] = x;
+      if (i % HD == 0) s.o.sum[row0 + i / HD] = total;
+    } else {
+      a.out[((int64_t)b * a.n_heads + gk * G) * HD + i] = __fdiv_rn(x, total);
+    }
   }
 }
 
@@ -767,7 +809,10 @@ constexpr size_t SMEM_MAX = 220 * 1024;
 // and none below 512 keys (b 1: at 128 keys 1 CTA 4.5 us, 4 CTAs 5.3 us; at 2048 keys 1 CTA 11.6 us, 16 CTAs
 // 5.8 us).  Split above 600 KB of codes an SM that has a CTA: at 262 KB (32 / 4 x 64, b 1, 32768 keys)
 // 13.4 us against 19.3 us split, at 1 MB (32 / 8 x 128, b 1, 32768 keys) 25.9 us against 24.6 us, at 2 MB
-// (16 / 16 x 128, b 1, 32768 keys) 51 us against 30 us.
+// (16 / 16 x 128, b 1, 32768 keys) 51 us against 30 us; but never where a sequence has at most 128 KB of codes
+// a head, for the split form's second launch and its waits then cost more than its larger ring gains
+// (32 / 8 x 128, b 256: at 512 keys 71 us against 95 us split, at 1024 keys 148 us against 126 us; 32 / 4 x 64,
+// b 256: at 1024 keys 41 us against 57 us, at 2048 keys 72 us against 65 us).
 struct ClusterPlan {
   int size, cap;
   size_t smem;
@@ -781,7 +826,9 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
   // clusters of 1, 2, 4, 8, 16 CTAs resident at once, by CTAs of all the shared memory and of half of it
   static int resident[64][2][5] = {};
   static bool ready[64] = {};
+  static std::mutex mu;
   if (device >= 64) return fail(SM_ERR_UNSUPPORTED, "attention_kv8: device id too large");
+  std::lock_guard<std::mutex> lock(mu);
   if (!ready[device]) {
     SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX));
     SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
@@ -800,7 +847,7 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
   }
   const int64_t bg = (int64_t)B * a.c.n_kv;
   const int64_t blocks = ((int64_t)a.prefix_len + 31) / 32 + ((int64_t)a.max_len + 31) / 32, keys = 32 * blocks;
-  plan.size = 0;
+  plan = {};
   for (int i = 4; i >= 0; --i) {
     const int cl = 1 << i;
     if (cl > 1 && (keys < 512 || cl * 128 > keys)) continue;
@@ -808,23 +855,23 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
     const size_t smem = M::bytes(cap);
     const int fit = resident[device][smem <= HALF][i];
     if (smem > SMEM_MAX || (cl > 1 && bg > fit)) continue;
-    const int64_t codes = bg * keys * 2 * HD, ctas = bg * cl;
-    if (codes / (ctas < sms ? ctas : sms) <= 600 * 1024) plan = {cl, (int)cap, smem};
+    const int64_t codes = keys * 2 * HD, ctas = bg * cl;
+    if (codes <= 128 * 1024 || bg * codes / (ctas < sms ? ctas : sms) <= 600 * 1024) plan = {cl, (int)cap, smem};
     break;
   }
   return SM_OK;
 }
 
 template <int HD, int GP>
-int launch_decode_cluster(const Kv8Attn& a, int B, const ClusterPlan& plan, cudaStream_t st) {
+int launch_decode_cluster(const Kv8Attn& a, const Kv8Behind& o, int B, const ClusterPlan& plan, cudaStream_t st) {
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = launch_config(dim3(plan.size, a.c.n_kv, B), DT, plan.smem, st, plan.size, attr);
-  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, decode_kv8_kernel<HD, GP>, a, plan.cap));
+  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, decode_kv8_kernel<HD, GP>, a, o, plan.cap));
   return SM_OK;
 }
 
 template <int HD, int GP>
-int launch_split(const Kv8Split& s, int B, bool pv, cudaStream_t st) {
+int launch_split_kernel(const Kv8Split& s, int B, bool pv, cudaStream_t st) {
   auto kern = pv ? split_pv_kernel<HD, GP> : split_scores_kernel<HD, GP>;
   const int smem = pv ? SplitSmem<HD, GP, true>::RING : SplitSmem<HD, GP, false>::RING;
   SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
@@ -836,50 +883,79 @@ int launch_split(const Kv8Split& s, int B, bool pv, cudaStream_t st) {
 
 int launch_split_as(const Kv8Split& s, int hd, int B, bool pv, cudaStream_t st) {
   if (hd == 64)
-    return s.gp == 4   ? launch_split<64, 4>(s, B, pv, st)
-           : s.gp == 8 ? launch_split<64, 8>(s, B, pv, st)
-                       : launch_split<64, 16>(s, B, pv, st);
-  return s.gp == 4   ? launch_split<128, 4>(s, B, pv, st)
-         : s.gp == 8 ? launch_split<128, 8>(s, B, pv, st)
-                     : launch_split<128, 16>(s, B, pv, st);
+    return s.gp == 4   ? launch_split_kernel<64, 4>(s, B, pv, st)
+           : s.gp == 8 ? launch_split_kernel<64, 8>(s, B, pv, st)
+                       : launch_split_kernel<64, 16>(s, B, pv, st);
+  return s.gp == 4   ? launch_split_kernel<128, 4>(s, B, pv, st)
+         : s.gp == 8 ? launch_split_kernel<128, 8>(s, B, pv, st)
+                     : launch_split_kernel<128, 16>(s, B, pv, st);
+}
+
+// Sizes the split form and returns the floats that its arrays take together.
+int64_t plan_split(Kv8Split& s, int hd, int B, int sms) {
+  const int G = s.a.n_heads / s.a.c.n_kv;
+  s.gp = G <= 4 ? 4 : G <= 8 ? 8 : 16;
+  const int64_t bg = (int64_t)B * s.a.c.n_kv;
+  // one wave of CTAs (2 an SM, or 1 where a group's accumulators fill the registers) where that makes chunks of
+  // 512 to 4096 keys (b 1, 131071 keys, 32 / 8 x 128: chunks of 1024 keys 87 us, of 2048 72 us, one wave of
+  // 3552 68 us)
+  const int ctas = s.gp == 4 || (hd == 64 && s.gp == 8) ? 2 : 1;
+  const int64_t wave = std::max<int64_t>(1, (int64_t)ctas * sms / bg);
+  s.chunk = (int)std::min<int64_t>(4096, std::max<int64_t>(512, ((s.a.max_len + wave - 1) / wave + 31) & ~31LL));
+  s.n_chunks = ceil_div(s.a.max_len, s.chunk);
+  const int64_t rows = bg * s.n_chunks;
+  return rows * s.chunk * s.gp + rows * s.gp * hd + rows * (2 * s.gp + 1) + bg;
+}
+
+int launch_split(Kv8Split& s, float* base, int hd, int B, cudaStream_t st) {
+  const int64_t rows = (int64_t)B * s.a.c.n_kv * s.n_chunks;
+  s.z = base;
+  s.pacc = s.z + rows * s.chunk * s.gp;
+  s.stat = s.pacc + rows * s.gp * hd;
+  s.arrived = (int*)(s.stat + rows * (2 * s.gp + 1));
+  SM_TRY(launch_split_as(s, hd, B, false, st));
+  return launch_split_as(s, hd, B, true, st);
 }
 
 int launch_decode_split(const Kv8Attn& a, int hd, int B, int sms, cudaStream_t st) {
   Kv8Split s = {};
   s.a = a;
   void* buf = nullptr;
-  if (cudaMallocAsync(&buf, (size_t)kv8_split_plan(s, hd, B, sms) * sizeof(float), st) != cudaSuccess) {
+  if (cudaMallocAsync(&buf, (size_t)plan_split(s, hd, B, sms) * sizeof(float), st) != cudaSuccess) {
     cudaGetLastError();
     return fail(SM_ERR_OOM, "attention_kv8: device allocation failed");
   }
-  kv8_split_place(s, hd, B, (float*)buf);
-  int rc = launch_split_as(s, hd, B, false, st);
-  if (rc == SM_OK) rc = launch_split_as(s, hd, B, true, st);
+  const int rc = launch_split(s, (float*)buf, hd, B, st);
   cudaFreeAsync(buf, st);
   return rc;
 }
 
-// The cluster form where it applies (plan.size > 0)
 template <int HD, int GP>
-int try_cluster(const Kv8Attn& a, int B, int device, int sms, cudaStream_t st, int* n_launch) {
-  ClusterPlan plan;
-  SM_TRY((plan_cluster<HD, GP>(a, B, device, sms, plan)));
-  *n_launch = plan.size ? 1 : 0;
-  return plan.size ? launch_decode_cluster<HD, GP>(a, B, plan, st) : SM_OK;
+struct ClusterForm {
+  static int plan(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& p) {
+    return plan_cluster<HD, GP>(a, B, device, sms, p);
+  }
+  static int launch(const Kv8Attn& a, const Kv8Behind& o, int B, const ClusterPlan& p, cudaStream_t st) {
+    return launch_decode_cluster<HD, GP>(a, o, B, p, st);
+  }
+};
+
+// f of the cluster form's instance for a head dim and group
+template <typename F>
+int with_cluster_form(int hd, int G, F f) {
+  if (hd == 64) return G <= 4 ? f(ClusterForm<64, 4>()) : G <= 8 ? f(ClusterForm<64, 8>()) : f(ClusterForm<64, 16>());
+  return G <= 4 ? f(ClusterForm<128, 4>()) : G <= 8 ? f(ClusterForm<128, 8>()) : f(ClusterForm<128, 16>());
 }
 
 int launch_decode(const Kv8Attn& a, int hd, int B, int device, int sms, cudaStream_t st, int* n_launch) {
-  const int G = a.n_heads / a.c.n_kv;
-  if (hd == 64)
-    SM_TRY(G <= 4   ? (try_cluster<64, 4>(a, B, device, sms, st, n_launch))
-           : G <= 8 ? (try_cluster<64, 8>(a, B, device, sms, st, n_launch))
-                    : (try_cluster<64, 16>(a, B, device, sms, st, n_launch)));
-  else
-    SM_TRY(G <= 4   ? (try_cluster<128, 4>(a, B, device, sms, st, n_launch))
-           : G <= 8 ? (try_cluster<128, 8>(a, B, device, sms, st, n_launch))
-                    : (try_cluster<128, 16>(a, B, device, sms, st, n_launch)));
-  if (*n_launch) return SM_OK;
-  if (a.prefix_len > 0) return launch_attention_shared_tc(a, hd, B, sms, st, n_launch);
+  ClusterPlan plan;
+  SM_TRY(with_cluster_form(hd, a.n_heads / a.c.n_kv, [&](auto form) {
+    SM_TRY(form.plan(a, B, device, sms, plan));
+    return plan.size ? form.launch(a, Kv8Behind{}, B, plan, st) : SM_OK;
+  }));
+  *n_launch = plan.size ? 1 : 0;
+  if (plan.size) return SM_OK;
+  if (a.prefix_len > 0) return launch_attention_shared_tc(a, hd, B, device, sms, st, n_launch);
   *n_launch = 2;
   return launch_decode_split(a, hd, B, sms, st);
 }
@@ -918,34 +994,32 @@ int check_attn(sm_ctx* ctx, const sm_kv8* c, const float* q, int64_t q_stride, c
 
 }  // namespace
 
-int64_t kv8_split_plan(Kv8Split& s, int hd, int B, int sms) {
-  const int G = s.a.n_heads / s.a.c.n_kv;
-  s.gp = G <= 4 ? 4 : G <= 8 ? 8 : 16;
-  const int64_t bg = (int64_t)B * s.a.c.n_kv;
-  // one wave of CTAs (2 an SM, or 1 where a group's accumulators fill the registers) where that makes chunks of
-  // 512 to 4096 keys (b 1, 131071 keys, 32 / 8 x 128: chunks of 1024 keys 87 us, of 2048 72 us, one wave of
-  // 3552 68 us)
-  const int ctas = s.gp == 4 || (hd == 64 && s.gp == 8) ? 2 : 1;
-  const int64_t wave = std::max<int64_t>(1, (int64_t)ctas * sms / bg);
-  s.chunk = (int)std::min<int64_t>(4096, std::max<int64_t>(512, ((s.a.max_len + wave - 1) / wave + 31) & ~31LL));
-  s.n_chunks = ceil_div(s.a.max_len, s.chunk);
-  const int64_t rows = bg * s.n_chunks;
-  return rows * s.chunk * s.gp + rows * s.gp * hd + rows * (2 * s.gp + 1) + bg;
+int plan_kv8_own(Kv8Own& own, int hd, int B, int device, int sms) {
+  ClusterPlan plan;
+  SM_TRY(with_cluster_form(hd, own.a.n_heads / own.a.c.n_kv,
+                           [&](auto form) { return form.plan(own.a, B, device, sms, plan); }));
+  own.cluster = plan.size;
+  own.cap = plan.cap;
+  own.smem = plan.smem;
+  Kv8Split s = {};
+  s.a = own.a;
+  own.floats = plan.size ? 0 : plan_split(s, hd, B, sms);
+  return SM_OK;
 }
 
-void kv8_split_place(Kv8Split& s, int hd, int B, float* base) {
-  const int64_t bg = (int64_t)B * s.a.c.n_kv, rows = bg * s.n_chunks;
-  s.z = base;
-  s.pacc = s.z + rows * s.chunk * s.gp;
-  s.stat = s.pacc + rows * s.gp * hd;
-  s.arrived = (int*)(s.stat + rows * (2 * s.gp + 1));
-}
-
-int launch_kv8_split_scores(const Kv8Split& s, int hd, int B, cudaStream_t st) {
-  return launch_split_as(s, hd, B, false, st);
-}
-int launch_kv8_split_pv(const Kv8Split& s, int hd, int B, cudaStream_t st) {
-  return launch_split_as(s, hd, B, true, st);
+int launch_kv8_own(const Kv8Own& own, float* workspace, int hd, int B, int sms, cudaStream_t st, int* n_launch) {
+  if (own.cluster) {
+    ++*n_launch;
+    return with_cluster_form(hd, own.a.n_heads / own.a.c.n_kv, [&](auto form) {
+      return form.launch(own.a, own.behind, B, ClusterPlan{own.cluster, own.cap, own.smem}, st);
+    });
+  }
+  *n_launch += 2;
+  Kv8Split s = {};
+  s.a = own.a;
+  s.o = own.behind;
+  plan_split(s, hd, B, sms);
+  return launch_split(s, workspace, hd, B, st);
 }
 
 }  // namespace sm

@@ -6,10 +6,9 @@
 //   prep    K and V codes -> fp16 tiles (codes are exact in fp16), query rows, scaled by a power of two into
 //           [-1, 1], -> fp16 pairs hi + lo (22 bits);
 //   max     S = (hi + lo) K^T per tile of 128 rows and block of 128 keys; row maxima of S * k_scale;
-//   own     (attn_kv8.cu) scores and maxima of the sequences' own keys;
+//   own     (attn_kv8.cu) the sequences' own keys, against the maximum of both parts;
 //   P V     S again, e against the maximum of both parts, P = e * v_scale relative to the prefix's largest
 //           scale as fp16 pairs hi + lo, O += (hi + lo) V;
-//   own     P V of the own keys;
 //   join    the parts' sums and weights, in order.
 // All products run as kind::f16 MMAs into fp32 TMEM accumulators; A (the query rows, then P, which takes the
 // place of the scores it came from) is in TMEM.  K and V tiles are laid out alike, in 128-byte-swizzled rows of
@@ -32,7 +31,7 @@ namespace {
 
 constexpr int QB = 128;          // query rows of a tile
 constexpr int KB = 128;          // keys of a block
-constexpr int SOFT_WARPS = 8;    // TMEM lane quarter = warp % 4, keys of a block: part warp / 4
+constexpr int SOFT_WARPS = 16;   // TMEM lane quarter = warp % 4, keys of a block: part warp / 4
 constexpr int SOFT = SOFT_WARPS * 32;
 constexpr int PARTS = SOFT_WARPS / 4;
 constexpr int PK = KB / PARTS;   // keys of a part
@@ -57,7 +56,9 @@ struct SharedArgs {
   float* v_top;             // [n_kv] the head's largest, at least 1e-30
   float* acc;               // [segment][128][HD], segment = CTA + n_kv * tile index (no two share one)
   float* sum;               // [segment][128]
-  Kv8Split own;             // the own keys (own.n_chunks == 0: none)
+  float* own_max;           // [n_kv][tiles * 128] largest own score, -inf where there is none
+  float* own_acc;           // [n_kv][tiles * 128][HD] the own keys' part; nullptr: nobody has any
+  float* own_sum;           // [n_kv][tiles * 128]
 };
 
 // ---------------------------------------------------------------- tcgen05 pieces
@@ -180,17 +181,8 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
   return *(const uint32_t*)&h;
 }
 
-// Largest of p and v in any order of the calls (v not NaN)
-__device__ __forceinline__ void atomic_max(float* p, float v) {
-  v += 0.f;  // -0 as 0
-  if (v >= 0.f)
-    atomicMax((int*)p, __float_as_int(v));
-  else
-    atomicMin((unsigned*)p, __float_as_uint(v));
-}
-
 // ---------------------------------------------------------------- prep
-// Blocks of the grid: K tiles, V tiles, query tiles.  Keys past the prefix and rows past the batch are zeros.
+// Blocks of the grid: K tiles, V tiles, parts of 16 rows of the query tiles.  Keys past the prefix and rows past the batch are zeros.
 template <int HD>
 __global__ void __launch_bounds__(256) shared_prep_kernel(SharedArgs s) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -236,11 +228,13 @@ __global__ void __launch_bounds__(256) shared_prep_kernel(SharedArgs s) {
     return;
   }
   id -= 2 * n_kt;
+  const int part = id % (QB / 16);
+  id /= QB / 16;
   const int g = id / s.tiles, tile = id - g * s.tiles;
   const int G = a.n_heads / a.c.n_kv;
   uint8_t* dst = s.qt + (int64_t)id * (2 * QB * HD * 2);
   constexpr int E = HD / 32;  // dims a lane
-  for (int r = tid >> 5; r < QB; r += 8) {
+  for (int r = part * 16 + (tid >> 5); r < part * 16 + 16; r += 8) {
     const int row = tile * QB + r;
     const int b = row / G, h = row - b * G;
     const bool live = row < s.rows && (!a.seq_ids || a.seq_ids[b] >= 0);
@@ -257,6 +251,7 @@ __global__ void __launch_bounds__(256) shared_prep_kernel(SharedArgs s) {
     if (lane == 0) {
       s.unit[(int64_t)id * QB + r] = ok ? pow2i(e - 1) * (HD == 64 ? 0.25f : 0.176776695f) : NAN;
       s.row_max[(int64_t)id * QB + r] = -INFINITY;
+      s.own_max[(int64_t)id * QB + r] = -INFINITY;
     }
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
@@ -509,16 +504,7 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
       } else {
         // the row's maximum over the prefix and the own keys
         const float unit = s.unit[row];
-        float m = s.row_max[row] * unit;
-        if (s.own.n_chunks && (tile % s.tiles) * QB + r < s.rows) {
-          const int G = a.n_heads / a.c.n_kv, at_row = (tile % s.tiles) * QB + r, b = at_row / G, h = at_row % G;
-          const int slot = a.seq_ids ? a.seq_ids[b] : b, len = a.lens[b];
-          if (slot >= 0 && slot < a.c.slots && len >= 0 && len <= a.max_len) {
-            const int used = (len + s.own.chunk - 1) / s.own.chunk;
-            const float* st = s.own.stat + ((int64_t)b * a.c.n_kv + g) * s.own.n_chunks * (2 * s.own.gp + 1) + h;
-            for (int c = 0; c < used; ++c) m = fmaxf(m, st[c * (2 * s.own.gp + 1)] * (unit * (1.f / 4194304.f)));
-          }
-        }
+        const float m = fmaxf(s.row_max[row] * unit, s.own_max[row]);
         const Pair unit2(unit), minus_m(-m);
         Pair sum2(0.f);
         // weights of 16 keys, P over their scores; TAIL: only the first `left` keys exist
@@ -631,35 +617,42 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
   }
 }
 
-// grid (n_heads, B), HD threads
-__global__ void shared_join_kernel(SharedArgs s) {
+// A thread: 4 dims of a row.  Grid: 256 threads, kv heads.
+template <int HD>
+__global__ void __launch_bounds__(256) shared_join_kernel(SharedArgs s) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const Kv8Attn& a = s.a;
-  const int head = blockIdx.x, b = blockIdx.y, d = threadIdx.x, HD = blockDim.x;
+  constexpr int L = HD / 4;
+  const int row = blockIdx.x * (256 / L) + threadIdx.x / L, d = threadIdx.x % L * 4, g = blockIdx.y;
+  if (row >= s.rows) return;
+  const int G = a.n_heads / a.c.n_kv, b = row / G, h = row - b * G;
   int slot, len;
   if (!row_keys(a, b, slot, len)) return;
-  const int G = a.n_heads / a.c.n_kv, g = head / G, h = head - g * G;
-  const int row = b * G + h, tile = g * s.tiles + row / QB, r = row % QB;
-  float x = 0.f, total = 0.f;
+  const int tile = g * s.tiles + row / QB, r = row % QB;
+  float4 x = {};
+  float total = 0.f;
+  auto add = [&](const float* acc, float sum) {
+    const float4 y = *(const float4*)(acc + d);
+    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+    total += sum;
+  };
   for (int c = tile * s.n_blocks / s.per; c <= ((tile + 1) * s.n_blocks - 1) / s.per; ++c) {
     const int64_t at = ((int64_t)c + tile) * QB + r;
-    x += s.acc[at * HD + d];
-    total += s.sum[at];
+    add(s.acc + at * HD, s.sum[at]);
   }
-  if (s.own.n_chunks) {
-    const int used = (len + s.own.chunk - 1) / s.own.chunk, gp = s.own.gp;
-    const int64_t own = ((int64_t)b * a.c.n_kv + g) * s.own.n_chunks;
-    for (int c = 0; c < used; ++c) {
-      x += s.own.pacc[((own + c) * gp + h) * HD + d];
-      total += s.own.stat[(own + c) * (2 * gp + 1) + gp + 1 + h];
-    }
+  if (s.own_acc) {
+    const int64_t at = (int64_t)tile * QB + r;
+    add(s.own_acc + at * HD, s.own_sum[at]);
   }
-  a.out[((int64_t)b * a.n_heads + head) * HD + d] = __fdiv_rn(x, total);
+  float* out = a.out + ((int64_t)b * a.n_heads + g * G + h) * HD + d;
+  out[0] = __fdiv_rn(x.x, total), out[1] = __fdiv_rn(x.y, total);
+  out[2] = __fdiv_rn(x.z, total), out[3] = __fdiv_rn(x.w, total);
 }
 
 template <int HD>
-int launch_shared(SharedArgs& s, int B, cudaStream_t st, int* n_launch) {
+int launch_shared(const SharedArgs& s, const Kv8Own& own, float* own_space, int B, int sms, cudaStream_t st,
+                  int* n_launch) {
   auto max_pass = shared_pass_kernel<HD, true>;
   auto pv_pass = shared_pass_kernel<HD, false>;
   constexpr size_t max_smem = TcSmem<HD, true>::BYTES, pv_smem = TcSmem<HD, false>::BYTES;
@@ -667,31 +660,22 @@ int launch_shared(SharedArgs& s, int B, cudaStream_t st, int* n_launch) {
   SM_CUDA_TRY(cudaFuncSetAttribute(pv_pass, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pv_smem));
   cudaLaunchAttribute attr[2];
   const int n_kv = s.a.c.n_kv;
-  cudaLaunchConfig_t cfg = launch_config(dim3(2 * n_kv * s.n_blocks + n_kv * s.tiles), 256, 0, st, 1, attr);
+  cudaLaunchConfig_t cfg = launch_config(dim3(2 * n_kv * s.n_blocks + n_kv * s.tiles * (QB / 16)), 256, 0, st, 1, attr);
   SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, shared_prep_kernel<HD>, s));
   cfg = launch_config(dim3(s.n_ctas), THREADS, max_smem, st, 1, attr);
   SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, max_pass, s));
-  *n_launch += 2;
-  if (s.own.n_chunks) {
-    SM_TRY(launch_kv8_split_scores(s.own, HD, B, st));
-    ++*n_launch;
-  }
+  if (s.own_acc) SM_TRY(launch_kv8_own(own, own_space, HD, B, sms, st, n_launch));
   cfg = launch_config(dim3(s.n_ctas), THREADS, pv_smem, st, 1, attr);
   SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, pv_pass, s));
-  ++*n_launch;
-  if (s.own.n_chunks) {
-    SM_TRY(launch_kv8_split_pv(s.own, HD, B, st));
-    ++*n_launch;
-  }
-  cfg = launch_config(dim3(s.a.n_heads, B), HD, 0, st, 1, attr);
-  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, shared_join_kernel, s));
-  ++*n_launch;
+  cfg = launch_config(dim3(ceil_div(s.rows, 1024 / HD), n_kv), 256, 0, st, 1, attr);
+  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, shared_join_kernel<HD>, s));
+  *n_launch += 4;
   return SM_OK;
 }
 
 }  // namespace
 
-int launch_attention_shared_tc(const Kv8Attn& a, int hd, int B, int sms, cudaStream_t st, int* n_launch) {
+int launch_attention_shared_tc(const Kv8Attn& a, int hd, int B, int device, int sms, cudaStream_t st, int* n_launch) {
   SharedArgs s = {};
   s.a = a;
   const int n_kv = a.c.n_kv;
@@ -701,17 +685,19 @@ int launch_attention_shared_tc(const Kv8Attn& a, int hd, int B, int sms, cudaStr
   s.rows = (int)rows;
   const int64_t tiles = (int64_t)n_kv * s.tiles, units = tiles * s.n_blocks;
   // unit, tile and grid indexes are 32-bit
-  if (units > (1 << 30) || 2ll * n_kv * s.n_blocks + tiles > (1 << 30))
+  if (units > (1 << 30) || 2ll * n_kv * s.n_blocks + tiles * (QB / 16) > (1 << 30))
     return fail(SM_ERR_SHAPE, "attention_shared_kv8: batch times prefix too large");
   s.per = ceil_div(units, std::min<int64_t>(sms, units));
   s.n_ctas = ceil_div(units, s.per);
-  s.own.a = a;
+  Kv8Own own = {};
+  own.a = a;
+  own.a.prefix_len = 0;
+  if (a.max_len > 0) SM_TRY(plan_kv8_own(own, hd, B, device, sms));
   const int64_t tile = 128ll * hd * 2, rp = tiles * QB, segments = s.n_ctas + tiles, blocks = (int64_t)n_kv * s.n_blocks;
-  const int64_t own = a.max_len > 0 ? kv8_split_plan(s.own, hd, B, sms) : 0;
   // every part in whole 16 bytes, the first ones in whole tiles
   const int64_t f_acc = segments * QB * hd, f_sum = segments * QB, f_scales = blocks * 2 * KB, f_vmax = blocks * 4,
-                f_top = (n_kv + 3) & ~3;
-  const int64_t bytes = (2 * blocks + 2 * tiles) * tile + (f_acc + f_sum + f_scales + 2 * rp + f_vmax + f_top + own) * 4;
+                f_top = (n_kv + 3) & ~3, f_own = a.max_len > 0 ? rp * hd + rp + own.floats : 0;
+  const int64_t bytes = (2 * blocks + 2 * tiles) * tile + (f_acc + f_sum + f_scales + 3 * rp + f_vmax + f_top + f_own) * 4;
   uint8_t* buf = nullptr;
   if (cudaMallocAsync((void**)&buf, (size_t)bytes, st) != cudaSuccess) {
     cudaGetLastError();
@@ -725,15 +711,18 @@ int launch_attention_shared_tc(const Kv8Attn& a, int hd, int B, int sms, cudaStr
   s.scales = s.sum + f_sum;
   s.unit = s.scales + f_scales;
   s.row_max = s.unit + rp;
-  s.v_max = s.row_max + rp;
+  s.own_max = s.row_max + rp;
+  s.v_max = s.own_max + rp;
   s.v_top = s.v_max + f_vmax;
-  if (own) {
-    kv8_split_place(s.own, hd, B, s.v_top + f_top);
-    s.own.prefix_max = s.row_max;
-    s.own.prefix_unit = s.unit;
-    s.own.prefix_rows = s.tiles * QB;
+  float* own_space = nullptr;
+  if (f_own) {
+    s.own_acc = s.v_top + f_top;
+    s.own_sum = s.own_acc + rp * hd;
+    own_space = s.own_sum + rp;
   }
-  const int rc = hd == 64 ? launch_shared<64>(s, B, st, n_launch) : launch_shared<128>(s, B, st, n_launch);
+  own.behind = {s.row_max, s.unit, s.tiles * QB, s.own_max, s.own_acc, s.own_sum};
+  const int rc = hd == 64 ? launch_shared<64>(s, own, own_space, B, sms, st, n_launch)
+                          : launch_shared<128>(s, own, own_space, B, sms, st, n_launch);
   cudaFreeAsync(buf, st);
   return rc;
 }

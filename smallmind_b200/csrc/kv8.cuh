@@ -72,29 +72,39 @@ __device__ __forceinline__ bool row_keys(const Kv8Attn& a, int b, int& slot, int
   return true;
 }
 
-// The long form of the decode attention (attn_kv8.cu): scores of chunks of keys, then P V.  Also the own keys
-// of the batch behind a shared prefix, whose maxima and sums then come from attn_kv8_tc.cu.
-struct Kv8Split {
-  Kv8Attn a;
-  int chunk, n_chunks;  // keys of a chunk (whole blocks of 32); chunks that max_len makes
-  int gp;               // heads a kv head's group is padded to: 4, 8 or 16
-  float* z;             // [B][n_kv][gp / 8 or 1][blocks] blocks of scores
-  float* pacc;          // [B][n_kv][n_chunks][gp][head_dim]
-  float* stat;          // [B][n_kv][n_chunks][2 * gp + 1] maxima, largest V scale; then the weights' sums
-  int* arrived;         // [B][n_kv] chunks whose P V is done
-  // behind a shared prefix: the largest raw score of row b * group + head, [n_kv][prefix_rows], and its factor
-  // (z = score * unit); the chunks are then joined by the caller
-  const float* prefix_max;
-  const float* prefix_unit;
-  int prefix_rows;
+// For the own keys of a batch behind a shared prefix (attn_kv8_tc.cu), row = kv head * rows + b * group + head:
+// what is known of the prefix's scores, and where the own part goes.
+struct Kv8Behind {
+  const float* prefix_max;   // nullptr: there is no such prefix
+  const float* prefix_unit;  // a row's largest score is prefix_max * prefix_unit
+  int rows;
+  float* own_max;            // largest own score, -inf at first
+  float* acc;                // [row][head_dim] sum of weights times values
+  float* sum;                // [row] sum of weights
 };
-// Sizes chunk, n_chunks and gp; returns the floats that z, pacc, stat and arrived take together.
-int64_t kv8_split_plan(Kv8Split& s, int head_dim, int B, int sms);
-void kv8_split_place(Kv8Split& s, int head_dim, int B, float* base);
-int launch_kv8_split_scores(const Kv8Split& s, int head_dim, int B, cudaStream_t st);
-int launch_kv8_split_pv(const Kv8Split& s, int head_dim, int B, cudaStream_t st);
+
+// Own-key attention behind a prefix: one launch or two; what they need beside the caller's arrays.
+struct Kv8Own {
+  Kv8Attn a;                 // prefix_len 0
+  Kv8Behind behind;
+  int cluster, cap;          // the cluster form's size and keys of a CTA; 0: the split form
+  size_t smem;
+  int64_t floats;            // the split form's workspace
+};
+int plan_kv8_own(Kv8Own& own, int head_dim, int B, int device, int sms);
+int launch_kv8_own(const Kv8Own& own, float* workspace, int head_dim, int B, int sms, cudaStream_t st, int* n_launch);
+
+// Larger of p and v into p, in any order of the calls; a NaN is dropped
+__device__ __forceinline__ void atomic_max(float* p, float v) {
+  v += 0.f;  // -0 as 0
+  if (v >= 0.f)
+    atomicMax((int*)p, __float_as_int(v));
+  else if (v < 0.f)
+    atomicMin((unsigned*)p, __float_as_uint(v));
+}
 
 // attn_kv8_tc.cu: decode attention behind a shared prefix (prefix_len > 0) on tcgen05
-int launch_attention_shared_tc(const Kv8Attn& a, int head_dim, int B, int sms, cudaStream_t st, int* n_launch);
+int launch_attention_shared_tc(const Kv8Attn& a, int head_dim, int B, int device, int sms, cudaStream_t st,
+                               int* n_launch);
 
 }  // namespace sm
