@@ -17,6 +17,13 @@
 // tile, block) units are dealt evenly to one CTA an SM; a CTA's units of one tile make a segment with sums of
 // its own.  The accumulation of O inside the tensor cores truncates: over 111 blocks it was 2e-5 off, so every
 // FLUSH blocks O moves on to fp32 sums in memory.
+//
+// Bound by the tensor cores: at fp32 accuracy a block takes 16 + 32 MMAs (head_dim 128) in the two passes, 64 clocks
+// each.  32 / 8 heads of 128, 256 rows over 32768 keys: max 95 us (82% of the time on the tensor pipe), P V 218 us
+// (72%: P of a block is waited for while both score buffers are taken), prep 33 us (HBM: 67 MB of codes in, 134 MB
+// of tiles out), own keys 67 us, join 10 us.  Four score buffers of 64 keys keep the pipe full, but an MMA of 64
+// columns takes as long as one of 128 (P V 238 us); two halves of the softmax warps that take every other block
+// 230 us; 8 softmax warps instead of 16 the same time.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -637,6 +644,7 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedArgs s) {
     x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
     total += sum;
   };
+#pragma unroll 4
   for (int c = tile * s.n_blocks / s.per; c <= ((tile + 1) * s.n_blocks - 1) / s.per; ++c) {
     const int64_t at = ((int64_t)c + tile) * QB + r;
     add(s.acc + at * HD, s.sum[at]);
