@@ -193,8 +193,9 @@ typedef struct sm_kv8 {
 } sm_kv8;
 
 /* All four calls below take device pointers and run on the context's stream without
- * synchronising; they can be captured into a CUDA graph.  A sequence id below 0 marks a padding row: nothing
- * is read, and what the row would have written is left as it was.  A sequence id,
+ * synchronising; they can be captured into a CUDA graph.  A sequence id below 0 marks a
+ * padding row: nothing of it is used, and what it would have written is left as it was
+ * (its place in k and v of sm_kv8_write has to be readable all the same).  A sequence id,
  * position or length outside the cache is reported as SM_ERR_SHAPE by
  * sm_ctx_device_status, and its row is treated like a padding row.  n_rows == 0 or
  * B == 0 does nothing. */
@@ -204,8 +205,8 @@ typedef struct sm_kv8 {
  * in floats, >= n_kv * head_dim, so rows may sit inside a fused Q|K|V row).
  * Per kv head: scale = max|x| * (1 / 127) in fp32, code = x / scale rounded to the
  * nearest integer, ties to even (exactly, whatever the magnitudes); a scale of 0
- * (zeros, or values that all round away) has codes 0.  A head with an infinity or NaN gets scale NaN and codes 0,
- * so it reads back as NaN.  Each (slot, position) at most once per call: what two
+ * (zeros, or values that all round away) has codes 0.  A head with an infinity or NaN
+ * gets scale NaN and codes 0, so it reads back as NaN.  Each (slot, position) at most once per call: what two
  * rows with the same target leave in it is unspecified. */
 SM_API int sm_kv8_write(sm_ctx* ctx, const sm_kv8* cache, const float* k, const float* v, int64_t row_stride,
                         const int* seq_ids, const int* positions, int n_rows);

@@ -56,7 +56,8 @@ __device__ __forceinline__ int zpos(int head, int g) { return head * 32 + (g & 3
 // q of one kv head's group as digits in B-fragment order; `unit` gets 2^(e - 22) / sqrt(HD) of this
 // lane's column head (lane / 4), the factor of its digit sums (NaN where q is not finite).
 template <int HD, int GP>
-__device__ __forceinline__ void load_q(const float* q, bool vec, int G, int lane, uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
+__device__ __forceinline__ void load_q(const float* q, bool vec, int G, int lane,
+                                       uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
                                        float (&unit)[Tile<HD, GP>::NT]) {
   using T = Tile<HD, GP>;
   const int g = lane >> 2, t = lane & 3;
@@ -102,7 +103,8 @@ struct KBlock {
 
 // Scores of a block: to z ([NT] planes `plane` floats apart), and this lane's running maxima of columns 2t, 2t + 1.
 template <int HD, int GP>
-__device__ __forceinline__ void score_block(const KBlock<HD>& k, const uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
+__device__ __forceinline__ void score_block(const KBlock<HD>& k,
+                                            const uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
                                             int g, int t, float* z, int64_t plane,
                                             float (&mx)[Tile<HD, GP>::NT][2]) {
   using T = Tile<HD, GP>;
@@ -121,7 +123,8 @@ __device__ __forceinline__ void score_block(const KBlock<HD>& k, const uint32_t 
         mma_s8s8(d[2], a0, a1, a2, a3, qd[nt][i][2][0], qd[nt][i][2][1]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[2 * m + (i >> 1)][i & 1] = join3_small(d[2][i], d[1][i], d[0][i]) * k.s[2 * m + (i >> 1)];
+      for (int i = 0; i < 4; ++i)
+        s[2 * m + (i >> 1)][i & 1] = join3_small(d[2][i], d[1][i], d[0][i]) * k.s[2 * m + (i >> 1)];
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -168,14 +171,16 @@ struct PVSum {
   }
 
   float m[T::NT], unit[T::NT], esum[T::NT];  // of this lane's head: maximum, factor of the scores, sum of weights
-  float mult, back;                          // fixed point: e = 1 at scale vmax is 2^23 - 8
+  float top, inv;                            // largest V scale and 1 / it
   int acc[T::MD][T::MT][4];
 
-  // Scales under 1e-30 keep the resolution of 1e-30, so that neither factor overflows.
+  // Fixed point: e = 1 at the largest scale is POINT = 2^23 - 8.  In two factors each way, so that none of them
+  // leaves the normal numbers; scales below those keep their resolution.
+  static constexpr float POINT = 8388600.f;
+  __device__ __forceinline__ float value(float sum) const { return sum * (1.f / POINT) * top; }
   __device__ __forceinline__ void start(float vmax, const float (&max_of)[T::NT], const float (&unit_of)[T::NT]) {
-    vmax = max_nan(vmax, 1e-30f);
-    mult = 8388600.f / vmax;
-    back = vmax * (1.f / 8388600.f);
+    top = max_nan(vmax, 0x1p-126f);
+    inv = 1.f / top;
 #pragma unroll
     for (int nt = 0; nt < T::NT; ++nt) unit[nt] = unit_of[nt], m[nt] = max_of[nt], esum[nt] = 0.f;
 #pragma unroll
@@ -190,7 +195,7 @@ struct PVSum {
   __device__ __forceinline__ void add(VBlock<HD, GP>& v, const float (&zv)[T::NT][NZ], int keys, int lane) {
     const int g = lane >> 2, t = lane & 3;
     const int first = T::PA ? t + (g >> 2) * 16 : t;
-    const float vsm = v.s * mult;
+    const float vsm = v.s * inv * POINT;
     uint32_t dg[T::NT][3][NZ / 4];
 #pragma unroll
     for (int nt = 0; nt < T::NT; ++nt) {
@@ -260,7 +265,7 @@ struct PVSum {
         float o[T::MT];
 #pragma unroll
         for (int c = 0; c < T::MT; ++c)
-          o[c] = join3(acc[0][c][2 + i], __shfl_xor_sync(0xffffffffu, acc[0][c][i], 16), acc[0][c][i]) * back;
+          o[c] = value(join3(acc[0][c][2 + i], __shfl_xor_sync(0xffffffffu, acc[0][c][i], 16), acc[0][c][i]));
         if (g < 4) {
 #pragma unroll
           for (int c = 0; c < T::MT; c += 4)
@@ -276,8 +281,8 @@ struct PVSum {
           for (int i = 0; i < 2; ++i) {
             float* p = to + (nt * 8 + 2 * t + i) * HD + d0 + g * T::VB + 2 * mt;
             *(float2*)p = make_float2(
-                join3(acc[3 * nt + 2][mt][i], acc[3 * nt + 1][mt][i], acc[3 * nt][mt][i]) * back,
-                join3(acc[3 * nt + 2][mt][i + 2], acc[3 * nt + 1][mt][i + 2], acc[3 * nt][mt][i + 2]) * back);
+                value(join3(acc[3 * nt + 2][mt][i], acc[3 * nt + 1][mt][i], acc[3 * nt][mt][i])),
+                value(join3(acc[3 * nt + 2][mt][i + 2], acc[3 * nt + 1][mt][i + 2], acc[3 * nt][mt][i + 2])));
           }
     }
   }
@@ -988,7 +993,8 @@ int check_attn(sm_ctx* ctx, const sm_kv8* c, const float* q, int64_t q_stride, c
   if (q_stride < (int64_t)n_heads * c->head_dim) return refuse(SM_ERR_SHAPE, "q_stride is less than a row");
   if (!seq_ids && B > c->max_seqs) return refuse(SM_ERR_SHAPE, "more rows than slots");
   if (!ctx || (B && (!q || !lens || !out))) return refuse(SM_ERR_INVALID_ARG, "null argument");
-  if (((uintptr_t)q | (uintptr_t)out) % 4) return refuse(SM_ERR_INVALID_ARG, "misaligned pointer");
+  if (((uintptr_t)q | (uintptr_t)out | (uintptr_t)seq_ids | (uintptr_t)lens) % 4)
+    return refuse(SM_ERR_INVALID_ARG, "misaligned pointer");
   return SM_OK;
 }
 
@@ -1034,7 +1040,8 @@ SM_API int sm_attention_decode_kv8(sm_ctx* ctx, const sm_kv8* cache, const float
   const char* what = "attention_decode_kv8";
   SM_TRY(check_attn(ctx, cache, q, q_stride, seq_ids, lens, max_len, B, n_heads, out, what));
   if (B == 0) return SM_OK;
-  Kv8Attn a{kv8_view(cache), {}, 0, 0, q, q_stride, seq_ids, lens, max_len, n_heads, out, nullptr, q_rows_vec(q, q_stride)};
+  Kv8Attn a{kv8_view(cache), {}, 0, 0, q, q_stride, seq_ids, lens, max_len, n_heads,
+            out, nullptr, q_rows_vec(q, q_stride)};
   return attend(ctx, a, cache->head_dim, B, what);
 }
 

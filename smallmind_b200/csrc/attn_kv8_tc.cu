@@ -60,7 +60,7 @@ struct SharedArgs {
   float* unit;              // [n_kv][tiles * 128] factor of a row's scores
   float* row_max;           // [n_kv][tiles * 128] largest S * k_scale
   float* v_max;             // [n_kv][n_blocks][4] largest V scales of 32 keys each
-  float* v_top;             // [n_kv] the head's largest, at least 1e-30
+  float* v_top;             // [n_kv] the head's largest, at least 2^-126
   float* acc;               // [segment][128][HD], segment = CTA + n_kv * tile index (no two share one)
   float* sum;               // [segment][128]
   float* own_max;           // [n_kv][tiles * 128] largest own score, -inf where there is none
@@ -189,7 +189,8 @@ __device__ __forceinline__ uint32_t pack_half(float a, float b) {
 }
 
 // ---------------------------------------------------------------- prep
-// Blocks of the grid: K tiles, V tiles, parts of 16 rows of the query tiles.  Keys past the prefix and rows past the batch are zeros.
+// Blocks of the grid: K tiles, V tiles, parts of 16 rows of the query tiles.  Keys past the prefix and rows past
+// the batch are zeros.
 template <int HD>
 __global__ void __launch_bounds__(256) shared_prep_kernel(SharedArgs s) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -244,7 +245,7 @@ __global__ void __launch_bounds__(256) shared_prep_kernel(SharedArgs s) {
   for (int r = part * 16 + (tid >> 5); r < part * 16 + 16; r += 8) {
     const int row = tile * QB + r;
     const int b = row / G, h = row - b * G;
-    const bool live = row < s.rows && (!a.seq_ids || a.seq_ids[b] >= 0);
+    const bool live = row < s.rows && row_in_range(a, b);
     const float* q = a.q + (int64_t)b * a.q_stride + (int64_t)(g * G + h) * HD + E * lane;
     float x[E];
     float peak = 0.f;
@@ -352,7 +353,8 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
         if (j >= NSC) ok = mbar_wait_bounded(&sc_free[sc.slot], sc.parity ^ 1, a.status);
         if (!ok) break;
         mbar_expect_tx(&sc_full[sc.slot], 2 * KB * 4);
-        bulk_g2s(smem + M::SCALES + sc.slot * (2 * KB * 4), s.scales + from * (2 * KB), 2 * KB * 4, &sc_full[sc.slot]);
+        bulk_g2s(smem + M::SCALES + sc.slot * (2 * KB * 4), s.scales + from * (2 * KB), 2 * KB * 4,
+                 &sc_full[sc.slot]);
         sc.next<NSC>();
         if constexpr (!MAX) {
           if (j >= M::NV) ok = mbar_wait_bounded(&v_free[v.slot], v.parity ^ 1, a.status);
@@ -441,7 +443,7 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
       const int n = a.c.n_kv * s.n_blocks, share = (n + gridDim.x - 1) / gridDim.x;
       for (int i = cta * share + warp; i < min(n, (cta + 1) * share); i += SOFT_WARPS) {
         const int g = i / s.n_blocks;
-        float m = 1e-30f;  // under it P keeps the resolution of 1e-30
+        float m = 0x1p-126f;  // 1 / m is finite
         for (int e = lane; e < s.n_blocks * 4; e += 32) m = max_nan(m, s.v_max[(int64_t)g * s.n_blocks * 4 + e]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -668,7 +670,8 @@ int launch_shared(const SharedArgs& s, const Kv8Own& own, float* own_space, int 
   SM_CUDA_TRY(cudaFuncSetAttribute(pv_pass, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pv_smem));
   cudaLaunchAttribute attr[2];
   const int n_kv = s.a.c.n_kv;
-  cudaLaunchConfig_t cfg = launch_config(dim3(2 * n_kv * s.n_blocks + n_kv * s.tiles * (QB / 16)), 256, 0, st, 1, attr);
+  const int prep = 2 * n_kv * s.n_blocks + n_kv * s.tiles * (QB / 16);
+  cudaLaunchConfig_t cfg = launch_config(dim3(prep), 256, 0, st, 1, attr);
   SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, shared_prep_kernel<HD>, s));
   cfg = launch_config(dim3(s.n_ctas), THREADS, max_smem, st, 1, attr);
   SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, max_pass, s));
@@ -701,11 +704,13 @@ int launch_attention_shared_tc(const Kv8Attn& a, int hd, int B, int device, int 
   own.a = a;
   own.a.prefix_len = 0;
   if (a.max_len > 0) SM_TRY(plan_kv8_own(own, hd, B, device, sms));
-  const int64_t tile = 128ll * hd * 2, rp = tiles * QB, segments = s.n_ctas + tiles, blocks = (int64_t)n_kv * s.n_blocks;
+  const int64_t tile = 128ll * hd * 2, rp = tiles * QB, segments = s.n_ctas + tiles;
+  const int64_t blocks = (int64_t)n_kv * s.n_blocks;
   // every part in whole 16 bytes, the first ones in whole tiles
   const int64_t f_acc = segments * QB * hd, f_sum = segments * QB, f_scales = blocks * 2 * KB, f_vmax = blocks * 4,
                 f_top = (n_kv + 3) & ~3, f_own = a.max_len > 0 ? rp * hd + rp + own.floats : 0;
-  const int64_t bytes = (2 * blocks + 2 * tiles) * tile + (f_acc + f_sum + f_scales + 3 * rp + f_vmax + f_top + f_own) * 4;
+  const int64_t bytes =
+      (2 * blocks + 2 * tiles) * tile + (f_acc + f_sum + f_scales + 3 * rp + f_vmax + f_top + f_own) * 4;
   uint8_t* buf = nullptr;
   if (cudaMallocAsync((void**)&buf, (size_t)bytes, st) != cudaSuccess) {
     cudaGetLastError();

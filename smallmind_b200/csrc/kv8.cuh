@@ -29,7 +29,7 @@ inline Kv8View kv8_view(const sm_kv8* c) {
 // none of it goes through __restrict__ or the read-only path, whose loads may move ahead of the wait.  attr
 // backs the result.
 inline cudaLaunchConfig_t launch_config(dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster,
-                                 cudaLaunchAttribute (&attr)[2]) {
+                                        cudaLaunchAttribute (&attr)[2]) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
@@ -70,6 +70,12 @@ __device__ __forceinline__ bool row_keys(const Kv8Attn& a, int b, int& slot, int
     return false;
   }
   return true;
+}
+
+// The same as a question
+__device__ __forceinline__ bool row_in_range(const Kv8Attn& a, int b) {
+  const int slot = a.seq_ids ? a.seq_ids[b] : b, len = a.lens[b];
+  return slot >= 0 && slot < a.c.slots && len >= 0 && len <= a.max_len;
 }
 
 // For the own keys of a batch behind a shared prefix (attn_kv8_tc.cu), row = kv head * rows + b * group + head:

@@ -84,7 +84,9 @@ struct Pair {
   __device__ __forceinline__ Pair() {}
   __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
   __device__ __forceinline__ explicit Pair(float a) : Pair(a, a) {}
-  __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+  __device__ __forceinline__ void get(float& a, float& b) const {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+  }
 };
 __device__ __forceinline__ Pair mul2(Pair a, Pair b) {
   Pair r;

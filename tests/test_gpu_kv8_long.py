@@ -174,3 +174,33 @@ def test_long_forms_in_two_graphs_at_once():
     torch.cuda.synchronize()
     for entry in graphs:
         entry[0].close()
+
+
+# (rows, own keys, prefix): one launch, split over the GPU, behind a short prefix, behind a long one
+FORMS = [(3, 300, 0), (3, 41000, 0), (3, 50, 200), (130, 40, 1000), (130, 700, 900)]
+
+
+@pytest.mark.parametrize("B,n,P", FORMS)
+@pytest.mark.parametrize("k_size,v_size,q_size", [(1e-20, 1e-33, 1e20), (1e25, 1e-37, 1e-26), (1, 1e30, 1),
+                                                  (1e-37, 1e-25, 1e36)])
+def test_magnitudes(ctx, B, n, P, k_size, v_size, q_size):
+    """Values near both ends of fp32's range: scores and results stay in it, so they are as exact as others.  (A
+    result in the subnormal range is a half step of that, 2^-150, off at most; so is each of its terms.)"""
+    rs = np.random.RandomState(B)
+    n_heads, n_kv, hd = (4, 1, 128) if n > 10000 else (16, 8, 128)
+    lens = rs.randint(n // 2, n + 1, B)
+    c = Cache(ctx, B, n, n_kv, hd).fill(rs, lens)
+    p = Cache(ctx, 1, max(P, 1), n_kv, hd).fill(rs, [P])
+    for x in (c, p):
+        x.ks *= k_size
+        x.vs *= v_size
+        x.vs[:, 0, 1::2] *= 1e-3
+    q = (rs.randn(B, n_heads, hd) * q_size).astype(np.float32)
+    q[0, 0] = 0
+    got = run_decode(ctx, c, q, None, lens, n, prefix=p if P else None, prefix_len=P)
+    a, pa = c.arrays(), p.arrays()
+    some = [0, 1, B - 1]
+    keys = [([(pa, 0, P)] if P else []) + [(a, b, lens[b])] for b in some]
+    want, tol = kv8_ref.attend_rows(q[some], n_kv, keys)
+    check(got[some], want, tol + 64 * 2.0 ** -150)
+    assert np.isfinite(got).all() and got.any()

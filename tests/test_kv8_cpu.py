@@ -53,6 +53,28 @@ def test_row_calls_refuse_bad_arguments():
         assert call() == -1 and "null" in last_error()  # the context
 
 
+@pytest.mark.parametrize("at", range(4))
+def test_row_calls_refuse_misaligned_pointers(at):
+    """Checked after the context, which therefore has to look like one; nothing of it is used."""
+    f, c = lib(), view()
+    p = [P] * 4
+    p[at] += 2
+    assert f.sm_kv8_write(P, c, p[0], p[1], 128, p[2], p[3], 1) == -1 and "misaligned" in last_error()
+    assert f.sm_kv8_read(P, c, p[2], p[3], 1, p[0], p[1], 128) == -1 and "misaligned" in last_error()
+
+
+@pytest.mark.parametrize("name", ["q", "seq", "lens", "out"])
+def test_attention_refuses_misaligned_pointers(name):
+    a = dict(q=P, seq=P, lens=P, out=P)
+    a[name] += 2
+    f = lib()
+    assert f.sm_attention_decode_kv8(P, view(), a["q"], 256, a["seq"], a["lens"], 32, 1, 4, a["out"]) == -1
+    assert "misaligned" in last_error()
+    assert f.sm_attention_shared_kv8(P, view(), 0, 1, view(), a["q"], 256, a["seq"], a["lens"], 32, 1, 4,
+                                     a["out"]) == -1
+    assert "misaligned" in last_error()
+
+
 @pytest.mark.parametrize("change,code", [
     (dict(B=-1), -2), (dict(n_heads=0), -2), (dict(n_heads=-2), -2), (dict(n_heads=5), -2), (dict(n_heads=34), -5),
     (dict(max_len=-1), -2), (dict(max_len=33), -2), (dict(stride=255), -2), (dict(seq=None, B=5), -2),
