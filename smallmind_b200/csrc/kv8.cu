@@ -12,6 +12,8 @@
 // takes 4 neighbouring values (16 bytes of fp32, 4 of codes), so every access of a warp is contiguous and a
 // head's maximum is one reduction over its 16 or 32 lanes.  What hides the latency is bytes on their way: a
 // warp takes several pieces of 128 values and starts all of their loads before it uses the first.
+#include <algorithm>
+
 #include "kv8.cuh"
 
 namespace sm {
@@ -73,8 +75,8 @@ __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float s) {
 // A warp's share: N pieces of 128 values, from piece N * (blockIdx.y / 2), of the K (even blockIdx.y) or V
 // values of row blockIdx.x * warps + warp.  Both sides are walked by constant steps.  Rows run fastest, so
 // CTAs that run together touch few heads (the other order: 8 to 13 % slower).  N measured with 8 heads of 128:
-// writing 32768 rows and reading them back with 1, 2, 4 pieces each 177, 134, 130 us; reading 65536 rows with
-// 1, 2, 4, 8 pieces 190, 131, 152, 205 us.
+// reading 65536 rows with 1, 2, 4, 8 pieces 190, 131, 152, 205 us (and 128 us at best with the next row's codes
+// loaded ahead, which is not done).
 template <int HD, int N>
 struct Share {
   int row, value, dim, left;  // row; this lane's first value in it; its dim; values from it to the row's end
@@ -95,56 +97,75 @@ struct Share {
   }
 };
 
+// CTAs of the write kernel an SM: what its registers allow.  The grid holds so many, and a warp starts the loads of
+// its next row before it quantises the one that has come (32768 rows of 8 heads of 128: 113 us, against 125 us
+// with a warp for every row; 2, 3, 4, 6 CTAs an SM 129, 113, 128, 115 us; with 1, 2, 8 pieces 133, 117, 115 us;
+// 100000 rows of 2 heads of 64: 60 us against 84 us).
+constexpr int write_ctas(int n) { return n == 4 ? 3 : 4; }
+
 template <int HD, int N, bool VEC>
-__global__ void __launch_bounds__(THREADS) kv8_write_kernel(Kv8View c, const float* k,
-                                                            const float* v, int64_t row_stride,
-                                                            const int* seq_ids,
-                                                            const int* positions, int n_rows,
-                                                            int* status) {
+__global__ void __launch_bounds__(THREADS, write_ctas(N))
+    kv8_write_kernel(Kv8View c, const float* k, const float* v, int64_t row_stride, const int* seq_ids,
+                     const int* positions, int n_rows, int* status) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Share<HD, N> w(c);
-  if (w.row >= n_rows) return;
-  const int slot = seq_ids[w.row], pos = positions[w.row];
-  const float* src = (w.is_v ? v : k) + w.row * row_stride + w.value;
+  const int step = gridDim.x * (THREADS / 32);
+  const float* src = (w.is_v ? v : k) + w.value;
   float x[N][4];
+  int slot = -1, pos = 0;
+  // the values do not wait for the ids to be checked (3 % slower)
+  auto load = [&](int64_t row) {
+    if (row >= n_rows) return;
+    slot = seq_ids[row], pos = positions[row];
+    const float* from = src + row * row_stride;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < N; ++i) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
-    if (w.left > i * 128) {
-      if (VEC) {
-        *(float4*)x[i] = __ldcs((const float4*)(src + i * 128));
-      } else {
+      for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
+      if (w.left > i * 128) {
+        if (VEC) {
+          *(float4*)x[i] = __ldcs((const float4*)(from + i * 128));
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[i][e] = src[i * 128 + e];
+          for (int e = 0; e < 4; ++e) x[i][e] = from[i * 128 + e];
+        }
       }
     }
-  }
-  // only now, so that the values do not wait for the ids (checked first: 3 % slower)
-  if (!in_cache(c, slot, pos, status)) return;
-  const int64_t at = w.at(c, slot, pos);
-  int8_t* codes = (w.is_v ? c.v : c.k) + at * HD + w.dim;
-  float* scales = (w.is_v ? c.vs : c.ks) + at;
+  };
+  load(w.row);
+  for (int64_t row = w.row; row < n_rows; row += step) {
+    float y[N][4];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    // the maximum as bits: non-negative floats order like integers, and infinities and NaNs lie above them
-    unsigned peak = 0;
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) peak = max(peak, __float_as_uint(x[i][e]) & 0x7fffffffu);
-    peak = __reduce_max_sync(HD == 128 ? 0xffffffffu : threadIdx.x % 32 < 16 ? 0xffffu : 0xffff0000u, peak);
-    if (w.left > i * 128) {
-      uint32_t word = 0;
-      float s = __uint_as_float(peak) * (1.f / 127.f);
-      if (peak >= 0x7f800000u)
-        s = __uint_as_float(0x7fffffffu);
-      else if (s > 0.f)
-        word = codes4(x[i], s);
-      *(uint32_t*)codes = word;
-      if (w.dim == 0) *scales = s;
+      for (int e = 0; e < 4; ++e) y[i][e] = x[i][e];
+    const int to_slot = slot, to_pos = pos;
+    load(row + step);
+    if (!in_cache(c, to_slot, to_pos, status)) continue;
+    const int64_t at = w.at(c, to_slot, to_pos);
+    int8_t* codes = (w.is_v ? c.v : c.k) + at * HD + w.dim;
+    float* scales = (w.is_v ? c.vs : c.ks) + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      // the maximum as bits: non-negative floats order like integers, and infinities and NaNs lie above them
+      unsigned peak = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) peak = max(peak, __float_as_uint(y[i][e]) & 0x7fffffffu);
+      peak = __reduce_max_sync(HD == 128 ? 0xffffffffu : threadIdx.x % 32 < 16 ? 0xffffu : 0xffff0000u, peak);
+      if (w.left > i * 128) {
+        uint32_t word = 0;
+        float s = __uint_as_float(peak) * (1.f / 127.f);
+        if (peak >= 0x7f800000u)
+          s = __uint_as_float(0x7fffffffu);
+        else if (s > 0.f)
+          word = codes4(y[i], s);
+        *(uint32_t*)codes = word;
+        if (w.dim == 0) *scales = s;
+      }
+      codes += w.step * HD;
+      scales += w.step;
     }
-    codes += w.step * HD;
-    scales += w.step;
   }
 }
 
@@ -220,7 +241,10 @@ SM_API int sm_kv8_write(sm_ctx* ctx, const sm_kv8* cache, const float* k, const 
   DeviceGuard guard(device);
   const Kv8View c = kv8_view(cache);
   const int pieces = ceil_div((int64_t)c.n_kv * cache->head_dim, 128), n = pieces >= 3 ? 4 : pieces;
-  const dim3 grid(ceil_div(n_rows, THREADS / 32), 2 * ceil_div(pieces, n));
+  const int parts = 2 * ceil_div(pieces, n);
+  int sms = 0;
+  SM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  const dim3 grid(std::min(ceil_div(n_rows, THREADS / 32), std::max(1, write_ctas(n) * sms / parts)), parts);
   const bool vec = rows_vectorizable(k, v, row_stride);
   const int which = (cache->head_dim == 64 ? 0 : 6) + (n == 4 ? 4 : 2 * (n - 1)) + vec;
   decltype(&kv8_write_kernel<64, 1, false>) const kernels[] = {
