@@ -14,8 +14,9 @@
 // place of the scores it came from) is in TMEM.  K and V tiles are laid out alike, in 128-byte-swizzled rows of
 // a key, and come by one bulk copy each (K as a K-major B operand, V as an MN-major one).  While the softmax
 // warps work on one block, the tensor cores form the next block's scores and the last block's P V.  The (row
-// tile, block) units are dealt evenly to one CTA an SM; a CTA's units of one tile make a segment with sums of
-// its own.  The accumulation of O inside the tensor cores truncates: over 111 blocks it was 2e-5 off, so every
+// tile, block) units are dealt evenly to one CTA an SM, so that CTAs with different row tiles walk the same blocks
+// together (they then come from L2: with 8 tiles of rows, each by itself, 747 MB came from HBM instead of 134); a
+// CTA's units of one tile make a segment with sums of its own.  The accumulation of O inside the tensor cores truncates: over 111 blocks it was 2e-5 off, so every
 // FLUSH blocks O moves on to fp32 sums in memory.
 //
 // Bound by the tensor cores: at fp32 accuracy a block takes 16 + 32 MMAs (head_dim 128) in the two passes, 64 clocks
@@ -53,7 +54,10 @@ struct SharedArgs {
   Kv8Attn a;
   int rows, tiles;          // query rows of a kv head, tiles of 128
   int n_blocks;             // blocks of 128 keys
-  int per, n_ctas;          // units of a CTA, in the order [n_kv][tile][block]; CTAs
+  // Units (tile, block) are dealt to groups of `ways` CTAs, which walk the same blocks at the same time with
+  // neighbouring tiles: a line of blocks belongs to `ways` tiles.  The lines lie behind one another, n_blocks each.
+  int ways, units;          // a divisor of tiles; blocks of all lines
+  int per, n_ctas;          // blocks of a CTA; CTAs
   uint8_t *kt, *vt;         // [n_kv][n_blocks] fp16 tiles [128 keys][HD]
   float* scales;            // [n_kv][n_blocks][K 128 | V 128]; past the prefix NaN | 0
   uint8_t* qt;              // [n_kv][tiles][hi | lo][128 rows][HD] fp16
@@ -61,12 +65,17 @@ struct SharedArgs {
   float* row_max;           // [n_kv][tiles * 128] largest S * k_scale
   float* v_max;             // [n_kv][n_blocks][4] largest V scales of 32 keys each
   float* v_top;             // [n_kv] the head's largest, at least 2^-126
-  float* acc;               // [segment][128][HD], segment = CTA + n_kv * tile index (no two share one)
+  float* acc;               // [segment][128][HD]; segment = CTA + tile of all kv heads, in lines (segment_of)
   float* sum;               // [segment][128]
   float* own_max;           // [n_kv][tiles * 128] largest own score, -inf where there is none
   float* own_acc;           // [n_kv][tiles * 128][HD] the own keys' part; nullptr: nobody has any
   float* own_sum;           // [n_kv][tiles * 128]
 };
+
+// A group's sums for a line of blocks, of one of its tiles; the groups and the lines both ascend, so no two share one
+__device__ __forceinline__ int64_t segment_of(const SharedArgs& s, int group, int line, int way) {
+  return ((int64_t)group + line) * s.ways + way;
+}
 
 // ---------------------------------------------------------------- tcgen05 pieces
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -314,8 +323,9 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
   uint32_t* tmem_slot = (uint32_t*)(v_free + M::NV);
   const Kv8Attn& a = s.a;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-  const int cta = blockIdx.x, units = a.c.n_kv * s.tiles * s.n_blocks;
-  const int u0 = cta * s.per, u1 = min(units, u0 + s.per);
+  const int group = blockIdx.x / s.ways, way = blockIdx.x - group * s.ways;
+  const int lines = s.tiles / s.ways;  // of a kv head
+  const int u0 = group * s.per, u1 = min(s.units, u0 + s.per);
 
   if (tid == 0) {
     mbar_init(q_full, SOFT_WARPS);
@@ -343,8 +353,8 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
       Ring k, v, sc;
       bool ok = true;
       for (int u = u0, j = 0; u < u1 && ok; ++u, ++j) {
-        const int tile = u / s.n_blocks;  // of all kv heads
-        const int64_t from = (int64_t)(tile / s.tiles) * s.n_blocks + (u - tile * s.n_blocks);
+        const int line = u / s.n_blocks;
+        const int64_t from = (int64_t)(line / lines) * s.n_blocks + (u - line * s.n_blocks);
         if (j >= M::NK) ok = mbar_wait_bounded(&k_free[k.slot], k.parity ^ 1, a.status);
         if (!ok) break;
         mbar_expect_tx(&k_full[k.slot], M::TILE);
@@ -441,7 +451,7 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
     if constexpr (MAX) {
       // this CTA's share of the V scales, relative to their head's largest (for the P V pass)
       const int n = a.c.n_kv * s.n_blocks, share = (n + gridDim.x - 1) / gridDim.x;
-      for (int i = cta * share + warp; i < min(n, (cta + 1) * share); i += SOFT_WARPS) {
+      for (int i = blockIdx.x * share + warp; i < min(n, ((int)blockIdx.x + 1) * share); i += SOFT_WARPS) {
         const int g = i / s.n_blocks;
         float m = 0x1p-126f;  // 1 / m is finite
         for (int e = lane; e < s.n_blocks * 4; e += 32) m = max_nan(m, s.v_max[(int64_t)g * s.n_blocks * 4 + e]);
@@ -456,7 +466,8 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
       }
     }
     for (int u = u0; u < u1;) {
-      const int tile = u / s.n_blocks, g = tile / s.tiles, blk0 = u - tile * s.n_blocks;
+      const int line = u / s.n_blocks, g = line / lines, blk0 = u - line * s.n_blocks;
+      const int tile = line * s.ways + way;  // of all kv heads
       const int nb = min(u1 - u, s.n_blocks - blk0);
       const int64_t row = (int64_t)tile * QB + r;
       {
@@ -547,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
           tmem_st8(cols + 8, lo);
         };
         // O of the blocks since the last flush into the segment's sums, which this thread alone adds to
-        const int64_t out = ((int64_t)cta + tile) * QB + r;
+        const int64_t out = segment_of(s, group, line, way) * QB + r;
         const float vmax = s.v_top[g];
         bool stored = false;
         auto flush = [&](const Ring& pb) {
@@ -646,9 +657,10 @@ __global__ void __launch_bounds__(256) shared_join_kernel(SharedArgs s) {
     x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
     total += sum;
   };
+  const int line = tile / s.ways, way = tile - line * s.ways;
 #pragma unroll 4
-  for (int c = tile * s.n_blocks / s.per; c <= ((tile + 1) * s.n_blocks - 1) / s.per; ++c) {
-    const int64_t at = ((int64_t)c + tile) * QB + r;
+  for (int c = line * s.n_blocks / s.per; c <= ((line + 1) * s.n_blocks - 1) / s.per; ++c) {
+    const int64_t at = segment_of(s, c, line, way) * QB + r;
     add(s.acc + at * HD, s.sum[at]);
   }
   if (s.own_acc) {
@@ -698,8 +710,16 @@ int launch_attention_shared_tc(const Kv8Attn& a, int hd, int B, int device, int 
   // unit, tile and grid indexes are 32-bit
   if (units > (1 << 30) || 2ll * n_kv * s.n_blocks + tiles * (QB / 16) > (1 << 30))
     return fail(SM_ERR_SHAPE, "attention_shared_kv8: batch times prefix too large");
-  s.per = ceil_div(units, std::min<int64_t>(sms, units));
-  s.n_ctas = ceil_div(units, s.per);
+  // as many ways as cost no more than 4 % in a CTA's blocks (256 rows over 32768 keys, sustained under the power
+  // limit: 1, 2, 4, 8 ways 470, 451, 442, 439 us for the whole call)
+  const int even = ceil_div(units, std::min<int64_t>(sms, units));
+  for (s.ways = std::min(sms, s.tiles);; --s.ways) {
+    if (s.tiles % s.ways) continue;
+    s.units = (int)(units / s.ways);
+    s.per = ceil_div(s.units, std::min(sms / s.ways, s.units));
+    if (s.ways == 1 || s.per <= even * 1.04) break;
+  }
+  s.n_ctas = ceil_div(s.units, s.per) * s.ways;
   Kv8Own own = {};
   own.a = a;
   own.a.prefix_len = 0;

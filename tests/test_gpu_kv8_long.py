@@ -115,6 +115,27 @@ def test_very_long_shared_prefix(ctx, n_heads, n_kv, hd, B, prefix_len):
     assert ctx.device_status() == 0
 
 
+@pytest.mark.parametrize("n_heads,n_kv,hd,B,prefix_len", [
+    (16, 1, 64, 1300, 700), (32, 4, 64, 150, 5003), (16, 2, 128, 210, 2500), (16, 1, 128, 2400, 130), (3, 3, 64, 901, 1111)])
+def test_many_tiles_of_query_rows(ctx, n_heads, n_kv, hd, B, prefix_len):
+    """More tiles of rows than processors, and numbers of tiles that divide evenly or not."""
+    rs = np.random.RandomState(B)
+    lens = rs.randint(0, 4, B)
+    p = Cache(ctx, 1, prefix_len, n_kv, hd).fill(rs, [prefix_len])
+    c = Cache(ctx, B, 3, n_kv, hd).fill(rs, lens)
+    q = rs.randn(B, n_heads, hd).astype(np.float32)
+    got = run_decode(ctx, c, q, None, lens, 3, prefix=p, prefix_len=prefix_len)
+    # the same rows in other tiles
+    shift = np.roll(np.arange(B), 37)
+    again = run_decode(ctx, c, q[shift], shift, lens[shift], 3, prefix=p, prefix_len=prefix_len)
+    a, pa = c.arrays(), p.arrays()
+    some = np.unique(np.r_[0, B - 1, rs.randint(0, B, 40)])
+    want, tol = kv8_ref.attend_rows(q[some], n_kv, [[(pa, 0, prefix_len), (a, b, lens[b])] for b in some])
+    check(got[some], want, tol)
+    check(again[np.argsort(shift)][some], want, tol)
+    assert ctx.device_status() == 0
+
+
 def test_long_forms_in_two_graphs_at_once():
     """The forms with workspaces (a shared prefix with split own keys, a split sequence) in graphs of two contexts
     on two streams, replayed side by side over changing lengths."""
