@@ -11,7 +11,8 @@
 // Both kernels are bound by HBM: a write moves 4 + 1 bytes a value and 4 a scale, a read the same.  A lane
 // takes 4 neighbouring values (16 bytes of fp32, 4 of codes), so every access of a warp is contiguous and a
 // head's maximum is one reduction over its 16 or 32 lanes.  What hides the latency is bytes on their way: a
-// warp takes several pieces of 128 values and starts all of their loads before it uses the first.
+// warp takes several pieces of 128 values and starts all of their loads before it uses the first.  (32768 rows of 8
+// heads of 128, written and read back: 111 us, floor 94 us; 65536 rows read: 111 us, floor 104 us.)
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -72,11 +73,9 @@ __device__ __forceinline__ uint32_t codes4(const float (&x)[4], float s) {
   return __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
 }
 
-// A warp's share: N pieces of 128 values, from piece N * (blockIdx.y / 2), of the K (even blockIdx.y) or V
+// A warp's share of a write: N pieces of 128 values, from piece N * (blockIdx.y / 2), of the K (even blockIdx.y) or V
 // values of row blockIdx.x * warps + warp.  Both sides are walked by constant steps.  Rows run fastest, so
-// CTAs that run together touch few heads (the other order: 8 to 13 % slower).  N measured with 8 heads of 128:
-// reading 65536 rows with 1, 2, 4, 8 pieces 190, 131, 152, 205 us (and 128 us at best with the next row's codes
-// loaded ahead, which is not done).
+// CTAs that run together touch few heads (the other order: 8 to 13 % slower).
 template <int HD, int N>
 struct Share {
   int row, value, dim, left;  // row; this lane's first value in it; its dim; values from it to the row's end
@@ -98,9 +97,9 @@ struct Share {
 };
 
 // CTAs of the write kernel an SM: what its registers allow.  The grid holds so many, and a warp starts the loads of
-// its next row before it quantises the one that has come (32768 rows of 8 heads of 128: 113 us, against 125 us
-// with a warp for every row; 2, 3, 4, 6 CTAs an SM 129, 113, 128, 115 us; with 1, 2, 8 pieces 133, 117, 115 us;
-// 100000 rows of 2 heads of 64: 60 us against 84 us).
+// its next row before it quantises the one that has come (32768 rows of 8 heads of 128, written and read back: 12 us
+// less than with a warp for every row; 2, 4, 6 CTAs an SM 16, 15, 2 us more than 3; with 1, 2, 8 pieces 20, 4,
+// 2 us more than with 4; 4 rows of one piece through shared memory, as in the read, 7 us more).
 constexpr int write_ctas(int n) { return n == 4 ? 3 : 4; }
 
 template <int HD, int N, bool VEC>
@@ -169,39 +168,57 @@ __global__ void __launch_bounds__(THREADS, write_ctas(N))
   }
 }
 
+// N pieces of 128 K or V values as above, of 4 rows a warp: a lane reads 16 neighbouring codes of one of them, so that
+// there are enough bytes on their way, and they pass through shared memory to come out as one row after the other, 4
+// values a lane (65536 rows of 8 heads of 128: with 1, 2, 4 pieces 115, 112, 111 us; 128 us with one row a warp, a
+// lane reading the 4 codes that it writes).
 template <int HD, int N, bool VEC>
-__global__ void __launch_bounds__(THREADS) kv8_read_kernel(Kv8View c, const int* seq_ids,
-                                                           const int* positions, int n_rows,
-                                                           float* k, float* v,
-                                                           int64_t row_stride, int* status) {
+__global__ void __launch_bounds__(THREADS) kv8_read_kernel(Kv8View c, const int* seq_ids, const int* positions,
+                                                           int n_rows, float* k, float* v, int64_t row_stride,
+                                                           int* status) {
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Share<HD, N> w(c);
-  float* to = w.is_v ? v : k;
-  if (w.row >= n_rows || !to) return;
-  const int slot = seq_ids[w.row], pos = positions[w.row];
-  if (!in_cache(c, slot, pos, status)) return;
-  const int64_t at = w.at(c, slot, pos);
-  const int8_t* codes = (w.is_v ? c.v : c.k) + at * HD + w.dim;
-  const float* scales = (w.is_v ? c.vs : c.ks) + at;
-  char4 q[N];
+  __shared__ int4 words[THREADS / 32][N][32];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t row0 = 4 * ((int64_t)blockIdx.x * (THREADS / 32) + warp), row = row0 + lane / 8;
+  const bool is_v = blockIdx.y & 1;
+  const int piece = (int)(blockIdx.y >> 1) * N, values = c.n_kv * HD;
+  float* to = is_v ? v : k;
+  if (row0 >= n_rows || !to) return;
+  int slot = -1, pos = 0;
+  if (row < n_rows) slot = seq_ids[row], pos = positions[row];
+  const bool live = in_cache(c, slot, pos, status);
+  const unsigned rows = __ballot_sync(0xffffffffu, live);
   float s[N];
+  int4 q[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-    if (w.left > i * 128) {
-      q[i] = *(const char4*)(codes + i * w.step * HD);
-      s[i] = scales[i * w.step];
+  for (int i = 0; i < N; ++i) {
+    const int value = (piece + i) * 128 + lane % 8 * 16;
+    s[i] = 0.f;
+    q[i] = make_int4(0, 0, 0, 0);
+    if (live && value < values) {
+      const int64_t at = c.at(slot, value / HD, pos);
+      q[i] = *(const int4*)((is_v ? c.v : c.k) + at * HD + value % HD);
+      s[i] = (is_v ? c.vs : c.ks)[at];
     }
-  to += w.row * row_stride + w.value;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) words[warp][i][lane] = q[i];
+  __syncwarp();
+  to += row0 * row_stride + piece * 128 + 4 * lane;
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    if (w.left > i * 128) {
-      const float4 y =
-          make_float4((float)q[i].x * s[i], (float)q[i].y * s[i], (float)q[i].z * s[i], (float)q[i].w * s[i]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const char4 x = ((const char4*)words[warp][i])[r * 32 + lane];
+      const float f = __shfl_sync(0xffffffffu, s[i], r * 8 + lane / 4);
+      if (!(rows >> (8 * r) & 1) || (piece + i) * 128 + 4 * lane >= values) continue;
+      float* out = to + r * row_stride + i * 128;
+      const float4 y = make_float4((float)x.x * f, (float)x.y * f, (float)x.z * f, (float)x.w * f);
       if (VEC) {
-        __stcs((float4*)(to + i * 128), y);
+        __stcs((float4*)out, y);
       } else {
-        to[i * 128] = y.x, to[i * 128 + 1] = y.y, to[i * 128 + 2] = y.z, to[i * 128 + 3] = y.w;
+        out[0] = y.x, out[1] = y.y, out[2] = y.z, out[3] = y.w;
       }
     }
 }
@@ -271,14 +288,15 @@ SM_API int sm_kv8_read(sm_ctx* ctx, const sm_kv8* cache, const int* seq_ids, con
   SM_TRY(ctx_view(ctx, &device, &st, &launches));
   DeviceGuard guard(device);
   const Kv8View c = kv8_view(cache);
-  const int pieces = ceil_div((int64_t)c.n_kv * cache->head_dim, 128), n = pieces >= 2 ? 2 : 1;
-  const dim3 grid(ceil_div(n_rows, THREADS / 32), 2 * ceil_div(pieces, n));
+  const int pieces = ceil_div((int64_t)c.n_kv * cache->head_dim, 128), n = pieces >= 3 ? 4 : pieces;
+  const dim3 grid(ceil_div(n_rows, 4 * (THREADS / 32)), 2 * ceil_div(pieces, n));
   const bool vec = rows_vectorizable(k, v, row_stride);
-  const int which = (cache->head_dim == 64 ? 0 : 4) + 2 * (n - 1) + vec;
+  const int which = (cache->head_dim == 64 ? 0 : 6) + (n == 4 ? 4 : 2 * (n - 1)) + vec;
   decltype(&kv8_read_kernel<64, 1, false>) const kernels[] = {
       kv8_read_kernel<64, 1, false>,  kv8_read_kernel<64, 1, true>,  kv8_read_kernel<64, 2, false>,
-      kv8_read_kernel<64, 2, true>,   kv8_read_kernel<128, 1, false>, kv8_read_kernel<128, 1, true>,
-      kv8_read_kernel<128, 2, false>, kv8_read_kernel<128, 2, true>};
+      kv8_read_kernel<64, 2, true>,   kv8_read_kernel<64, 4, false>, kv8_read_kernel<64, 4, true>,
+      kv8_read_kernel<128, 1, false>, kv8_read_kernel<128, 1, true>, kv8_read_kernel<128, 2, false>,
+      kv8_read_kernel<128, 2, true>,  kv8_read_kernel<128, 4, false>, kv8_read_kernel<128, 4, true>};
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = launch_config(grid, THREADS, 0, st, 1, attr);
   SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernels[which], c, seq_ids, positions, n_rows, k, v, row_stride,
