@@ -170,8 +170,8 @@ __global__ void __launch_bounds__(THREADS, write_ctas(N))
 
 // N pieces of 128 K or V values as above, of 4 rows a warp: a lane reads 16 neighbouring codes of one of them, so that
 // there are enough bytes on their way, and they pass through shared memory to come out as one row after the other, 4
-// values a lane (65536 rows of 8 heads of 128: with 1, 2, 4 pieces 115, 112, 111 us; 128 us with one row a warp, a
-// lane reading the 4 codes that it writes).
+// values a lane (65536 rows of 8 heads of 128: 112 us; 128 us with one row a warp, a lane reading the 4 codes that it
+// writes).
 template <int HD, int N, bool VEC>
 __global__ void __launch_bounds__(THREADS) kv8_read_kernel(Kv8View c, const int* seq_ids, const int* positions,
                                                            int n_rows, float* k, float* v, int64_t row_stride,
@@ -288,15 +288,19 @@ SM_API int sm_kv8_read(sm_ctx* ctx, const sm_kv8* cache, const int* seq_ids, con
   SM_TRY(ctx_view(ctx, &device, &st, &launches));
   DeviceGuard guard(device);
   const Kv8View c = kv8_view(cache);
-  const int pieces = ceil_div((int64_t)c.n_kv * cache->head_dim, 128), n = pieces >= 3 ? 4 : pieces;
-  const dim3 grid(ceil_div(n_rows, 4 * (THREADS / 32)), 2 * ceil_div(pieces, n));
+  const int pieces = ceil_div((int64_t)c.n_kv * cache->head_dim, 128), groups = ceil_div(n_rows, 4 * (THREADS / 32));
+  int sms = 0;
+  SM_CUDA_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  // two pieces a warp once that leaves 32 CTAs an SM (2500 rows of 8 heads of 128: 1 piece 4.6 us, 2 pieces 6.0 us;
+  // 65536 rows: 115 and 112 us)
+  const int n = (int64_t)groups * pieces >= 32ll * sms ? 2 : 1;
+  const dim3 grid(groups, 2 * ceil_div(pieces, n));
   const bool vec = rows_vectorizable(k, v, row_stride);
-  const int which = (cache->head_dim == 64 ? 0 : 6) + (n == 4 ? 4 : 2 * (n - 1)) + vec;
+  const int which = (cache->head_dim == 64 ? 0 : 4) + 2 * (n - 1) + vec;
   decltype(&kv8_read_kernel<64, 1, false>) const kernels[] = {
       kv8_read_kernel<64, 1, false>,  kv8_read_kernel<64, 1, true>,  kv8_read_kernel<64, 2, false>,
-      kv8_read_kernel<64, 2, true>,   kv8_read_kernel<64, 4, false>, kv8_read_kernel<64, 4, true>,
-      kv8_read_kernel<128, 1, false>, kv8_read_kernel<128, 1, true>, kv8_read_kernel<128, 2, false>,
-      kv8_read_kernel<128, 2, true>,  kv8_read_kernel<128, 4, false>, kv8_read_kernel<128, 4, true>};
+      kv8_read_kernel<64, 2, true>,   kv8_read_kernel<128, 1, false>, kv8_read_kernel<128, 1, true>,
+      kv8_read_kernel<128, 2, false>, kv8_read_kernel<128, 2, true>};
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg = launch_config(grid, THREADS, 0, st, 1, attr);
   SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernels[which], c, seq_ids, positions, n_rows, k, v, row_stride,

@@ -197,6 +197,40 @@ def test_long_forms_in_two_graphs_at_once():
         entry[0].close()
 
 
+@pytest.mark.parametrize("n,n_kv,hd,offset", [(40001, 9, 64, 0), (38011, 5, 128, 1), (70003, 1, 64, 0), (9000, 2, 64, 2)])
+def test_many_rows_there_and_back(ctx, n, n_kv, hd, offset):
+    """More rows than the warps that walk them, a half piece at the end of a row, padding among them."""
+    import torch
+    rs = np.random.RandomState(n)
+    slots, tokens = 7, n // 7 + 3
+    place = rs.permutation(slots * tokens)[:n]
+    seq, pos = (place // tokens).astype(np.int32), (place % tokens).astype(np.int32)
+    seq[::101] = -1
+    live = seq >= 0
+    w = n_kv * hd
+    stride = w + offset
+    x = rs.randn(2, n, w).astype(np.float32)
+    rows = np.zeros((2, n, stride), np.float32)
+    rows[:, :, :w] = x
+    c = Cache(ctx, slots, tokens, n_kv, hd)
+    d, ds, dp = dev(rows), dev(seq), dev(pos)
+    out = torch.full((2, n, stride), 7.0, device="cuda")
+    torch.cuda.synchronize()
+    c.h.write_device(d[0].data_ptr(), d[1].data_ptr(), ds.data_ptr(), dp.data_ptr(), n, row_stride=stride)
+    c.h.read_device(ds.data_ptr(), dp.data_ptr(), n, out[0].data_ptr(), out[1].data_ptr(), row_stride=stride)
+    assert ctx.device_status() == 0
+    codes, scale = kv8_ref.quantize(x.reshape(2, n, n_kv, hd))
+    want = np.full((2, n, stride), 7.0, np.float32)
+    want[:, live, :w] = (codes * scale[..., None]).reshape(2, n, w)[:, live]
+    assert np.array_equal(out.cpu().numpy(), want)
+    k, ks, v, vs = c.arrays()
+    free = np.ones((slots, tokens), bool)
+    free[seq[live], pos[live]] = False
+    for a in (k, v):
+        assert (a.transpose(0, 2, 1, 3)[free] == 55).all()
+    assert np.isnan(ks.transpose(0, 2, 1)[free]).all() and np.isnan(vs.transpose(0, 2, 1)[free]).all()
+
+
 # (rows, own keys, prefix): one launch, split over the GPU, behind a short prefix, behind a long one
 FORMS = [(3, 300, 0), (3, 41000, 0), (3, 50, 200), (130, 40, 1000), (130, 700, 900)]
 
