@@ -198,7 +198,8 @@ typedef struct sm_kv8 {
  * (its place in k and v of sm_kv8_write has to be readable all the same).  A sequence id,
  * position or length outside the cache is reported as SM_ERR_SHAPE by
  * sm_ctx_device_status, and its row is treated like a padding row.  n_rows == 0 or
- * B == 0 does nothing. */
+ * B == 0 does nothing.  The attention calls take their workspaces, where long contexts
+ * need any, from the device's stream-ordered pool (SM_ERR_OOM where it is exhausted). */
 
 /* Quantise K and V rows into the cache: row i goes to position positions[i] of slot
  * seq_ids[i].  k, v: row i at k + i * row_stride, [n_kv][head_dim] fp32 (row_stride
