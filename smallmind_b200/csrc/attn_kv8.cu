@@ -560,6 +560,7 @@ struct Kv8Split {
   float* z;             // [B][n_kv][gp / 8 or 1][blocks] blocks of scores
   float* pacc;          // [B][n_kv][n_chunks][gp][head_dim]
   float* stat;          // [B][n_kv][n_chunks][2 * gp + 1] maxima, largest V scale; then the weights' sums
+  float* unit;          // [B][n_kv][gp] factors of the heads' scores
   int* arrived;         // [B][n_kv] chunks whose P V is done
 };
 
@@ -642,6 +643,7 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, false>::CTAS)) split_sc
 #pragma unroll
     for (int i = 0; i < DW; ++i) m = fmaxf(m, wred[i][tid]);
     stat[tid] = m;
+    if (ch == 0) s.unit[bg * GP + tid] = unit_of[tid];
     if (s.o.prefix_max && tid < G)
       atomic_max(s.o.own_max + (int64_t)gk * s.o.rows + (int64_t)b * G + tid, m * unit_of[tid]);
   } else if (tid == GP) {
@@ -695,25 +697,12 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
   for (int i = 0; i < M::N - 1; ++i)
     if (32 * (tw + T::TW * i) < n)
       S::fetch(ring_at + i * S::BYTES, vp, nullptr, vsp, 32 * (tw + T::TW * i), n, lane, policy);
-  // the maximum over the sequence's chunks, and the factors of the heads
+  // the maximum over the sequence's chunks
   PVSum<HD, GP> pv;
   const int col = pv.column(g);
   float* stat = s.stat + bg * s.n_chunks * (2 * GP + 1);
   const int used = (len + s.chunk - 1) / s.chunk;
   float max_of[T::NT], unit[T::NT];
-#pragma unroll
-  for (int nt = 0; nt < T::NT; ++nt) {
-    // as load_q forms it
-    const float* q = a.q + (int64_t)b * a.q_stride + (int64_t)(gk * G + nt * 8 + col) * HD;
-    float peak = 0.f;
-    if (nt * 8 + col < G) {
-#pragma unroll 8
-      for (int i = t; i < HD; i += 4) peak = max_nan(peak, fabsf(q[i]));
-    }
-    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
-    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
-    unit[nt] = peak < INFINITY ? pow2i(block_exp(peak) - 22) * (HD == 64 ? 0.125f : 0.0883883476f) : NAN;
-  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
 #pragma unroll
@@ -728,6 +717,8 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
     gmax[warp][lane] = m;
   }
   const float vmax = stat[ch * (2 * GP + 1) + GP];
+#pragma unroll
+  for (int nt = 0; nt < T::NT; ++nt) unit[nt] = s.unit[bg * GP + nt * 8 + col];
   __syncthreads();
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) {
@@ -909,7 +900,7 @@ int64_t plan_split(Kv8Split& s, int hd, int B, int sms) {
   s.chunk = (int)std::min<int64_t>(4096, std::max<int64_t>(512, ((s.a.max_len + wave - 1) / wave + 31) & ~31LL));
   s.n_chunks = ceil_div(s.a.max_len, s.chunk);
   const int64_t rows = bg * s.n_chunks;
-  return rows * s.chunk * s.gp + rows * s.gp * hd + rows * (2 * s.gp + 1) + bg;
+  return rows * s.chunk * s.gp + rows * s.gp * hd + rows * (2 * s.gp + 1) + bg * s.gp + bg;
 }
 
 int launch_split(Kv8Split& s, float* base, int hd, int B, cudaStream_t st) {
@@ -917,7 +908,8 @@ int launch_split(Kv8Split& s, float* base, int hd, int B, cudaStream_t st) {
   s.z = base;
   s.pacc = s.z + rows * s.chunk * s.gp;
   s.stat = s.pacc + rows * s.gp * hd;
-  s.arrived = (int*)(s.stat + rows * (2 * s.gp + 1));
+  s.unit = s.stat + rows * (2 * s.gp + 1);
+  s.arrived = (int*)(s.unit + (int64_t)B * s.a.c.n_kv * s.gp);
   SM_TRY(launch_split_as(s, hd, B, false, st));
   return launch_split_as(s, hd, B, true, st);
 }
