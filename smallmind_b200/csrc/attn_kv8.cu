@@ -466,20 +466,20 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   vmax = warp_max_nan(vmax);
   if (lane == 0) vred[warp] = vmax;
   __syncthreads();
+  float m = -INFINITY;
   if (tid < GP) {
-    float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < DW; ++i) m = fmaxf(m, wred[i][tid]);
     stat[tid] = m;
   }
 #pragma unroll
   for (int i = 0; i < DW; ++i) vmax = max_nan(vmax, vred[i]);
-  cluster.sync();
-  if (tid < GP) {
-    float m = -INFINITY;
-    for (int r = 0; r < CL; ++r) m = fmaxf(m, cluster.map_shared_rank(stat, r)[tid]);
-    gmax[tid] = m;
+  if (CL > 1) {
+    cluster.sync();
+    if (tid < GP)
+      for (int r = 0; r < CL; ++r) m = fmaxf(m, cluster.map_shared_rank(stat, r)[tid]);
   }
+  if (tid < GP) gmax[tid] = m;
   __syncthreads();
 
   PVSum<HD, GP> pv;
@@ -515,18 +515,26 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   float* part = (float*)smem;  // [TW][GP][HD]
   pv.store(part + tw * GP * HD, wred[tw], lane, d0);
   __syncthreads();
-  if (tid < GP) {
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < T::TW; ++i) s += wred[i][tid];
-    stat[GP + tid] = s;
-  }
+  auto write = [&](int i, float s, float total) {
+    if (o.prefix_max) {
+      o.acc[row0 * HD + i] = s;
+      if (i % HD == 0) o.sum[row0 + i / HD] = total;
+    } else {
+      out[i] = __fdiv_rn(s, total);
+    }
+  };
   for (int i = tid; i < G * HD; i += DT) {
-    float s = 0.f;
+    float s = 0.f, total = 0.f;
 #pragma unroll
-    for (int r = 0; r < T::TW; ++r) s += part[r * GP * HD + i];
-    pacc[i] = s;
+    for (int r = 0; r < T::TW; ++r) s += part[r * GP * HD + i], total += wred[r][i / HD];
+    if (CL == 1) {
+      write(i, s, total);
+    } else {
+      pacc[i] = s;
+      if (i % HD == 0) stat[GP + i / HD] = total;
+    }
   }
+  if (CL == 1) return;
   cluster.sync();
   // each rank its share of the outputs
   for (int i = rank * DT + tid; i < G * HD; i += CL * DT) {
@@ -535,12 +543,7 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
       s += cluster.map_shared_rank(pacc, r)[i];
       total += cluster.map_shared_rank(stat, r)[GP + i / HD];
     }
-    if (o.prefix_max) {
-      o.acc[row0 * HD + i] = s;
-      if (i % HD == 0) o.sum[row0 + i / HD] = total;
-    } else {
-      out[i] = __fdiv_rn(s, total);
-    }
+    write(i, s, total);
   }
   cluster.sync();  // no CTA's shared memory goes before the others have read it
 }
