@@ -804,14 +804,17 @@ constexpr size_t SMEM_MAX = 220 * 1024;
 //
 // Size: CTAs of one cluster have to be resident together, and a second wave of clusters waits for whole
 // groups of SMs, so the largest size is taken whose clusters are all resident at once (32 / 4 heads of 64,
-// 16 rows of up to 1024 keys: 4 CTAs 7.3 us, 8 CTAs, which are not, 13.2 us), with 128 keys a CTA at least
-// and none below 512 keys (b 1: at 128 keys 1 CTA 4.5 us, 4 CTAs 5.3 us; at 2048 keys 1 CTA 11.6 us, 16 CTAs
-// 5.8 us).  Split above 600 KB of codes an SM that has a CTA: at 262 KB (32 / 4 x 64, b 1, 32768 keys)
-// 13.4 us against 19.3 us split, at 1 MB (32 / 8 x 128, b 1, 32768 keys) 25.9 us against 24.6 us, at 2 MB
-// (16 / 16 x 128, b 1, 32768 keys) 51 us against 30 us; but never where a sequence has at most 128 KB of codes
-// a head, for the split form's second launch and its waits then cost more than its larger ring gains
-// (32 / 8 x 128, b 256: at 512 keys 71 us against 95 us split, at 1024 keys 148 us against 126 us; 32 / 4 x 64,
-// b 256: at 1024 keys 41 us against 57 us, at 2048 keys 72 us against 65 us).
+// 16 rows of up to 1024 keys: 4 CTAs 7.7 us, 8 CTAs, which are not, 13.6 us), with 128 keys a CTA at least
+// and none up to 512 keys (32 / 4 x 64, 8 rows: at 512 keys 1 CTA 5.8 us, 4 CTAs 6.8 us; at 2048 keys 1 CTA 12 us,
+// 8 CTAs 7.7 us), nor 2 CTAs below 2048 keys of 128 dims (32 / 8 x 128, 16 rows of 1024: 1 CTA 10.3 us, 2 CTAs
+// 12.1 us).
+//
+// Split above 600 KB of codes an SM that has a CTA: at 262 KB (32 / 4 x 64, b 1, 32768 keys) 14.7 us against 18.3 us
+// split, at 1 MB (32 / 8 x 128, b 1, 32768 keys) 29 us against 23 us, at 2 MB (16 / 16 x 128, b 1, 32768 keys) 54 us
+// against 29 us; but never where a sequence has at most 128 KB of codes a head, for the split form's second launch
+// and its waits then cost more than its larger ring gains (32 / 8 x 128, b 256: at 512 keys 66 us against 87 us
+// split, at 1024 keys 138 us against 118 us; 32 / 4 x 64, b 256: at 1024 keys 39 us against 54 us, at 2048 keys 74 us
+// against 69 us).
 struct ClusterPlan {
   int size, cap;
   size_t smem;
@@ -820,10 +823,10 @@ struct ClusterPlan {
 template <int HD, int GP>
 int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan) {
   using M = ClusterSmem<HD, GP>;
-  constexpr size_t HALF = 113 * 1024;  // of an SM's shared memory, so that two CTAs fit
   auto kern = decode_kv8_kernel<HD, GP>;
-  // clusters of 1, 2, 4, 8, 16 CTAs resident at once, by CTAs of all the shared memory and of half of it
+  // clusters of 1, 2, 4, 8, 16 CTAs resident at once, by CTAs of all the shared memory and of what fits twice
   static int resident[64][2][5] = {};
+  static size_t twice[64] = {};
   static bool ready[64] = {};
   static std::mutex mu;
   if (device >= 64) return fail(SM_ERR_UNSUPPORTED, "attention_kv8: device id too large");
@@ -831,10 +834,17 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
   if (!ready[device]) {
     SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX));
     SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    cudaFuncAttributes fa;
+    int per_sm = 0, reserved = 0;
+    SM_CUDA_TRY(cudaFuncGetAttributes(&fa, kern));
+    SM_CUDA_TRY(cudaDeviceGetAttribute(&per_sm, cudaDevAttrMaxSharedMemoryPerMultiprocessor, device));
+    SM_CUDA_TRY(cudaDeviceGetAttribute(&reserved, cudaDevAttrReservedSharedMemoryPerBlock, device));
+    twice[device] = (per_sm / 2 - reserved - fa.sharedSizeBytes) & ~(size_t)127;
     for (int half = 0; half < 2; ++half)
       for (int i = 0; i < 5; ++i) {
         cudaLaunchAttribute attr[2];
-        cudaLaunchConfig_t probe = launch_config(dim3(1 << i), DT, half ? HALF : SMEM_MAX, nullptr, 1 << i, attr);
+        const size_t smem = half ? twice[device] : SMEM_MAX;
+        cudaLaunchConfig_t probe = launch_config(dim3(1 << i), DT, smem, nullptr, 1 << i, attr);
         int fit = 0;
         if (cudaOccupancyMaxActiveClusters(&fit, (const void*)kern, &probe) != cudaSuccess) {
           cudaGetLastError();
@@ -849,10 +859,11 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
   plan = {};
   for (int i = 4; i >= 0; --i) {
     const int cl = 1 << i;
-    if (cl > 1 && (keys < 512 || cl * 128 > keys)) continue;
+    if (cl > 1 && (keys <= 512 || cl * 128 > keys)) continue;
+    if (cl == 2 && HD == 128 && keys < 2048) continue;
     const int64_t cap = 32 * ((blocks + cl - 1) / cl);
     const size_t smem = M::bytes(cap);
-    const int fit = resident[device][smem <= HALF][i];
+    const int fit = resident[device][smem <= twice[device]][i];
     if (smem > SMEM_MAX || (cl > 1 && bg > fit)) continue;
     const int64_t codes = keys * 2 * HD, ctas = bg * cl;
     if (codes <= 128 * 1024 || bg * codes / (ctas < sms ? ctas : sms) <= 600 * 1024) plan = {cl, (int)cap, smem};
@@ -896,8 +907,8 @@ int64_t plan_split(Kv8Split& s, int hd, int B, int sms) {
   s.gp = G <= 4 ? 4 : G <= 8 ? 8 : 16;
   const int64_t bg = (int64_t)B * s.a.c.n_kv;
   // one wave of CTAs (2 an SM, or 1 where a group's accumulators fill the registers) where that makes chunks of
-  // 512 to 4096 keys (b 1, 131071 keys, 32 / 8 x 128: chunks of 1024 keys 87 us, of 2048 72 us, one wave of
-  // 3552 68 us)
+  // 512 to 4096 keys (b 1, 131071 keys, 32 / 8 x 128: chunks of 1024 keys 76 us, of 2048 62 us, one wave of
+  // 3552 54 us; b 64, 4096 to 8192 keys: of 1024 193 us, of 2048 159 us, of 4096 154 us)
   const int ctas = s.gp == 4 || (hd == 64 && s.gp == 8) ? 2 : 1;
   const int64_t wave = std::max<int64_t>(1, (int64_t)ctas * sms / bg);
   s.chunk = (int)std::min<int64_t>(4096, std::max<int64_t>(512, ((s.a.max_len + wave - 1) / wave + 31) & ~31LL));

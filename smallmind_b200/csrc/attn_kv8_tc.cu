@@ -15,9 +15,9 @@
 // a key, and come by one bulk copy each (K as a K-major B operand, V as an MN-major one).  While the softmax
 // warps work on one block, the tensor cores form the next block's scores and the last block's P V.  The (row
 // tile, block) units are dealt evenly to one CTA an SM, so that CTAs with different row tiles walk the same blocks
-// together (they then come from L2: with 8 tiles of rows, each by itself, 747 MB came from HBM instead of 134); a
-// CTA's units of one tile make a segment with sums of its own.  The accumulation of O inside the tensor cores truncates: over 111 blocks it was 2e-5 off, so every
-// FLUSH blocks O moves on to fp32 sums in memory.
+// together (they then come from L2: with 8 tiles of rows, each by itself, 747 MB came from HBM instead of 144); a
+// CTA's units of one tile make a segment with sums of its own.  The accumulation of O inside the tensor cores
+// truncates: over 111 blocks it was 2e-5 off, so every FLUSH blocks O moves on to fp32 sums in memory.
 //
 // Bound by the tensor cores: at fp32 accuracy a block takes 16 + 32 MMAs (head_dim 128) in the two passes, 64 clocks
 // each.  32 / 8 heads of 128, 256 rows over 32768 keys: max 95 us (82% of the time on the tensor pipe), P V 218 us

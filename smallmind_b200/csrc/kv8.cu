@@ -168,10 +168,10 @@ __global__ void __launch_bounds__(THREADS, write_ctas(N))
   }
 }
 
-// N pieces of 128 K or V values as above, of 4 rows a warp: a lane reads 16 neighbouring codes of one of them, so that
-// there are enough bytes on their way, and they pass through shared memory to come out as one row after the other, 4
-// values a lane (65536 rows of 8 heads of 128: 112 us; 128 us with one row a warp, a lane reading the 4 codes that it
-// writes).
+// N pieces of 128 K or V values as above, of 4 rows a warp: a lane reads 16 neighbouring codes of one of them, so
+// that there are enough bytes on their way, and they pass through shared memory to come out as one row after the
+// other, 4 values a lane (65536 rows of 8 heads of 128: 112 us; 128 us with one row a warp, a lane reading the 4
+// codes that it writes).
 template <int HD, int N, bool VEC>
 __global__ void __launch_bounds__(THREADS) kv8_read_kernel(Kv8View c, const int* seq_ids, const int* positions,
                                                            int n_rows, float* k, float* v, int64_t row_stride,
