@@ -814,7 +814,10 @@ constexpr size_t SMEM_MAX = 220 * 1024;
 // against 29 us; but never where a sequence has at most 128 KB of codes a head, for the split form's second launch
 // and its waits then cost more than its larger ring gains (32 / 8 x 128, b 256: at 512 keys 66 us against 87 us
 // split, at 1024 keys 138 us against 118 us; 32 / 4 x 64, b 256: at 1024 keys 39 us against 54 us, at 2048 keys 74 us
-// against 69 us).
+// against 69 us).  Behind a shared prefix, which L2 holds, the other form is attn_kv8_tc.cu, whose five launches
+// take 30 to 40 us at least where head_dim is 128: there the bound is 1056 KB (32 / 8 x 128, prefix of 4096: 16 rows,
+// 1056 KB, 28 us against 40 us; prefix of 1024: 64 rows, 1024 KB, 43 us against 41 us; 32 / 4 x 64, prefix of 4096,
+// 64 rows, 950 KB: 42 us against 32 us).
 struct ClusterPlan {
   int size, cap;
   size_t smem;
@@ -866,7 +869,8 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
     const int fit = resident[device][smem <= twice[device]][i];
     if (smem > SMEM_MAX || (cl > 1 && bg > fit)) continue;
     const int64_t codes = keys * 2 * HD, ctas = bg * cl;
-    if (codes <= 128 * 1024 || bg * codes / (ctas < sms ? ctas : sms) <= 600 * 1024) plan = {cl, (int)cap, smem};
+    const int64_t most = a.prefix_len > 0 && HD == 128 ? 1056 * 1024 : 600 * 1024;
+    if (codes <= 128 * 1024 || bg * codes / (ctas < sms ? ctas : sms) <= most) plan = {cl, (int)cap, smem};
     break;
   }
   return SM_OK;
