@@ -224,8 +224,8 @@ SM_API int sm_kv8_read(sm_ctx* ctx, const sm_kv8* cache, const int* seq_ids, con
  * q + b * q_stride, [n_heads][head_dim]; out: [B][n_heads * head_dim].
  * 0 <= lens[b] <= max_len <= max_tokens; a row of length 0 gives zeros.  max_len
  * sizes the launch, so a graph captured with it serves every shorter length.
- * n_heads is a multiple of n_kv, at most 16 q heads per kv head.  A NaN in q or in
- * a visible scale makes the outputs that depend on it NaN. */
+ * n_heads is a multiple of n_kv, at most 16 q heads per kv head; B is at most 65535.
+ * A NaN in q or in a visible scale makes the outputs that depend on it NaN. */
 SM_API int sm_attention_decode_kv8(sm_ctx* ctx, const sm_kv8* cache, const float* q, int64_t q_stride,
                                    const int* seq_ids, const int* lens, int max_len, int B, int n_heads,
                                    float* out);
