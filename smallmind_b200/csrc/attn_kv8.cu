@@ -29,8 +29,8 @@ namespace {
 //           the warp's keys, in the registers that the MMA wants them in; V codes are made
 //           fragments by 4 x 4 byte transposes.  With up to 4 heads the three digits of all of
 //           them are rows of one A operand; with more, a digit is a B operand of 8 heads.
-constexpr int DT = 256;
-constexpr int DW = DT / 32;
+// The kernels come with W = 8 and with W = 4 warps a CTA: twice as many of the smaller CTAs hide one another's phases
+// better once there are more of them than an SM holds.
 
 template <int HD, int GP>
 struct Tile {
@@ -39,13 +39,11 @@ struct Tile {
   static constexpr int CP = GP > 8 ? 8 : GP;    // heads a tile keeps
   static constexpr int ZB = 32 * CP;            // scores of a block and column tile
   static constexpr int DS = HD == 128 && GP == 16 ? 2 : 1;  // warps that split the dims of a key block
-  static constexpr int TW = DW / DS;            // warps that split the keys
   static constexpr int DP = HD / DS;            // dims a warp
   static constexpr int VB = DP / 8;             // bytes of a V row a lane
   // accumulator tiles: PA one for each byte of a lane (8 dims), else 16 dims x (heads, digits)
   static constexpr int MT = PA ? VB : DP / 16;
   static constexpr int MD = PA ? 1 : 3 * NT;
-  static constexpr int PART = TW * GP * HD;     // floats of the warps' sums
 };
 
 // Scores of a block lie as [head][t][8]: the scores of keys t + 4 i, i = 0..7, in a row.
@@ -376,22 +374,29 @@ __device__ __forceinline__ float warp_max_nan(float v) {
 // memory.  Behind a prefix (o) the weights are formed against the larger of both maxima and the sums are left to
 // be joined.  A warp's K blocks and then its V blocks go through one ring, so V is on its way while the maxima
 // are exchanged.  Bound by its chain of phases.
+// CTAs of W warps an SM: what a group's accumulators leave registers for
 template <int HD, int GP>
+constexpr int ctas_by_registers(int W) {
+  return (GP == 4 || (HD == 64 && GP == 8) ? 16 : 8) / W;
+}
+
+template <int HD, int GP, int W>
 struct ClusterSmem {
   using T = Tile<HD, GP>;
   using S = Slot<HD, GP, false>;
   static constexpr int N = HD == 64 ? 4 : 3;     // ring slots
-  static constexpr int RING = DW * N * S::BYTES;
+  static constexpr int RING = W * N * S::BYTES;
   static constexpr int TAIL = GP * HD + 2 * GP;  // this CTA's sums, maxima and weights for the cluster
-  static_assert(RING >= T::PART * 4, "the warps' sums take the rings' place");
+  static_assert(RING >= W / T::DS * GP * HD * 4, "the warps' sums take the rings' place");
   static size_t bytes(int64_t cap) { return RING + ((size_t)cap * GP + TAIL) * sizeof(float); }
 };
 
-template <int HD, int GP>
-__global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1)
+template <int HD, int GP, int W>
+__global__ void __launch_bounds__(32 * W, ctas_by_registers<HD, GP>(W))
     decode_kv8_kernel(Kv8Attn a, Kv8Behind o, int cap) {
   using T = Tile<HD, GP>;
-  using M = ClusterSmem<HD, GP>;
+  using M = ClusterSmem<HD, GP, W>;
+  constexpr int DW = W, DT = 32 * W, TW = W / T::DS;
   using S = Slot<HD, GP, false>;
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
@@ -430,14 +435,14 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   };
   // the warp's blocks: K blocks warp, warp + DW, ..; then V blocks tw, tw + TW, ..
   const int tw = warp / T::DS, d0 = (warp % T::DS) * T::DP;
-  const int nk = (blocks - warp + DW - 1) / DW, nv = (blocks - tw + T::TW - 1) / T::TW;
+  const int nk = (blocks - warp + DW - 1) / DW, nv = (blocks - tw + TW - 1) / TW;
   const uint8_t* ring = smem + warp * M::N * S::BYTES;
   const uint32_t ring_at = smem_u32(ring);
   const uint64_t once = l2_evict_first_policy(), often = l2_evict_normal_policy();
   auto fetch = [&](int i) {
     if (i < nk + nv) {
       const bool is_k = i < nk;
-      const int blk = b0 + (is_k ? warp + DW * i : tw + T::TW * (i - nk));
+      const int blk = b0 + (is_k ? warp + DW * i : tw + TW * (i - nk));
       const bool shared = blk < np;
       const Kv8View& c = shared ? a.prefix : a.c;
       const int64_t at = shared ? prefix0 : own0;
@@ -497,7 +502,7 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   }
   pv.start(vmax, max_of, unit);
   for (int i = nk; i < nk + nv; ++i) {
-    const int blk = tw + T::TW * (i - nk);
+    const int blk = tw + TW * (i - nk);
     cp_wait<M::N - 2>();
     VBlock<HD, GP> v;
     S::read_v(ring + i % M::N * S::BYTES, v, keys_of(blk), d0, lane);
@@ -526,7 +531,7 @@ __global__ void __launch_bounds__(DT, (GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1
   for (int i = tid; i < G * HD; i += DT) {
     float s = 0.f, total = 0.f;
 #pragma unroll
-    for (int r = 0; r < T::TW; ++r) s += part[r * GP * HD + i], total += wred[r][i / HD];
+    for (int r = 0; r < TW; ++r) s += part[r * GP * HD + i], total += wred[r][i / HD];
     if (CL == 1) {
       write(i, s, total);
     } else {
@@ -560,6 +565,7 @@ struct Kv8Split {
   Kv8Behind o;
   int chunk, n_chunks;  // keys of a chunk (whole blocks); chunks that max_len makes
   int gp;               // heads a kv head's group is padded to: 4, 8 or 16
+  int warps;            // of a CTA: 4 or 8
   float* z;             // [B][n_kv][gp / 8 or 1][blocks] blocks of scores
   float* pacc;          // [B][n_kv][n_chunks][gp][head_dim]
   float* stat;          // [B][n_kv][n_chunks][2 * gp + 1] maxima, largest V scale; then the weights' sums
@@ -567,22 +573,23 @@ struct Kv8Split {
   int* arrived;         // [B][n_kv] chunks whose P V is done
 };
 
-template <int HD, int GP, bool PV>
+template <int HD, int GP, int W, bool PV>
 struct SplitSmem {
   using S = Slot<HD, GP, PV>;
-  static constexpr int CTAS = PV ? ((GP == 4 || (HD == 64 && GP == 8)) ? 2 : 1) : (GP == 16 ? 1 : 2);
+  static constexpr int CTAS = PV ? ctas_by_registers<HD, GP>(W) : (GP == 16 ? 8 : 16) / W;
   // as many slots as the CTAs of an SM have room for
-  static constexpr int FIT = (CTAS == 2 ? 112 : 220) * 1024 / (DW * S::BYTES);
+  static constexpr int FIT = 224 / CTAS * 1024 / (W * S::BYTES);
   static constexpr int N = FIT > 6 ? 6 : FIT;
-  static constexpr int RING = DW * N * S::BYTES;
-  static_assert(N >= 3 && RING >= Tile<HD, GP>::PART * 4, "ring too small");
+  static constexpr int RING = W * N * S::BYTES;
+  static_assert(N >= 3 && RING >= W / Tile<HD, GP>::DS * GP * HD * 4, "ring too small");
 };
 
-template <int HD, int GP>
-__global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, false>::CTAS)) split_scores_kernel(Kv8Split s) {
+template <int HD, int GP, int W>
+__global__ void __launch_bounds__(32 * W, (SplitSmem<HD, GP, W, false>::CTAS)) split_scores_kernel(Kv8Split s) {
   using T = Tile<HD, GP>;
   using S = Slot<HD, GP, false>;
-  using M = SplitSmem<HD, GP, false>;
+  using M = SplitSmem<HD, GP, W, false>;
+  constexpr int DW = W;
   const Kv8Attn& a = s.a;
   const int ch = blockIdx.x, gk = blockIdx.y, b = blockIdx.z;
   const int G = a.n_heads / a.c.n_kv;
@@ -656,11 +663,12 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, false>::CTAS)) split_sc
   }
 }
 
-template <int HD, int GP>
-__global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_kernel(Kv8Split s) {
+template <int HD, int GP, int W>
+__global__ void __launch_bounds__(32 * W, (SplitSmem<HD, GP, W, true>::CTAS)) split_pv_kernel(Kv8Split s) {
   using T = Tile<HD, GP>;
   using S = Slot<HD, GP, true>;
-  using M = SplitSmem<HD, GP, true>;
+  using M = SplitSmem<HD, GP, W, true>;
+  constexpr int DW = W, DT = 32 * W, TW = W / T::DS;
   const Kv8Attn& a = s.a;
   const int ch = blockIdx.x, gk = blockIdx.y, b = blockIdx.z;
   const int G = a.n_heads / a.c.n_kv;
@@ -698,8 +706,8 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
   const uint64_t policy = l2_evict_first_policy();
 #pragma unroll
   for (int i = 0; i < M::N - 1; ++i)
-    if (32 * (tw + T::TW * i) < n)
-      S::fetch(ring_at + i * S::BYTES, vp, nullptr, vsp, 32 * (tw + T::TW * i), n, lane, policy);
+    if (32 * (tw + TW * i) < n)
+      S::fetch(ring_at + i * S::BYTES, vp, nullptr, vsp, 32 * (tw + TW * i), n, lane, policy);
   // the maximum over the sequence's chunks
   PVSum<HD, GP> pv;
   const int col = pv.column(g);
@@ -710,7 +718,7 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
   asm volatile("griddepcontrol.launch_dependents;");
 #pragma unroll
   for (int i = 0; i < M::N - 1; ++i) {
-    const int row = 32 * (tw + T::TW * i);
+    const int row = 32 * (tw + TW * i);
     if (row < n) S::fetch_scores(ring_at + i * S::BYTES, z, plane, row, lane);
     cp_commit();  // the first group holds all of the codes so far
   }
@@ -736,7 +744,7 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
   }
   pv.start(vmax, max_of, unit);
   int at = 0;
-  for (int row = 32 * tw; row < n; row += 32 * T::TW) {
+  for (int row = 32 * tw; row < n; row += 32 * TW) {
     cp_wait<M::N - 2>();
     const uint8_t* p = ring + at * S::BYTES;
     float zv[T::NT][pv.NZ];
@@ -747,7 +755,7 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
         *(float4*)&zv[nt][i] = *((const float4*)(p + S::MORE) + (nt * T::ZB + pv.zstart(g, t) + i) / 4);
     VBlock<HD, GP> v;
     S::read_v(p, v, n - row, d0, lane);
-    const int next = row + 32 * T::TW * (M::N - 1);
+    const int next = row + 32 * TW * (M::N - 1);
     if (next < n) {
       const uint32_t to = ring_at + (at == 0 ? M::N - 1 : at - 1) * S::BYTES;
       S::fetch(to, vp, nullptr, vsp, next, n, lane, policy);
@@ -766,13 +774,13 @@ __global__ void __launch_bounds__(DT, (SplitSmem<HD, GP, true>::CTAS)) split_pv_
   for (int i = tid; i < G * HD; i += DT) {
     float x = 0.f;
 #pragma unroll
-    for (int r = 0; r < T::TW; ++r) x += part[r * GP * HD + i];
+    for (int r = 0; r < TW; ++r) x += part[r * GP * HD + i];
     pacc[i] = x;
   }
   if (tid < GP) {
     float x = 0.f;
 #pragma unroll
-    for (int i = 0; i < T::TW; ++i) x += wred[i][tid];
+    for (int i = 0; i < TW; ++i) x += wred[i][tid];
     stat[ch * (2 * GP + 1) + GP + 1 + tid] = x;
   }
   // the last CTA of this (sequence, kv head) joins the chunks, always in their order
@@ -809,24 +817,29 @@ constexpr size_t SMEM_MAX = 220 * 1024;
 // 8 CTAs 7.7 us), nor 2 CTAs below 2048 keys of 128 dims (32 / 8 x 128, 16 rows of 1024: 1 CTA 10.3 us, 2 CTAs
 // 12.1 us).
 //
+// 4 warps a CTA instead of 8 where there is more than one wave of them and three (with many heads two) fit an SM
+// (b 256, at 256 keys: 32 / 8 x 128 38 us against 53 us, 32 / 4 x 64 13 us against 19 us; but b 64, which is less than
+// a wave, 7.4 us against 6.2 us).
+//
 // Split above 600 KB of codes an SM that has a CTA: at 262 KB (32 / 4 x 64, b 1, 32768 keys) 14.7 us against 18.3 us
 // split, at 1 MB (32 / 8 x 128, b 1, 32768 keys) 29 us against 23 us, at 2 MB (16 / 16 x 128, b 1, 32768 keys) 54 us
-// against 29 us; but never where a sequence has at most 128 KB of codes a head, for the split form's second launch
-// and its waits then cost more than its larger ring gains (32 / 8 x 128, b 256: at 512 keys 66 us against 87 us
-// split, at 1024 keys 138 us against 118 us; 32 / 4 x 64, b 256: at 1024 keys 39 us against 54 us, at 2048 keys 74 us
-// against 69 us).  Behind a shared prefix, which L2 holds, the other form is attn_kv8_tc.cu, whose five launches
-// take 30 to 40 us at least where head_dim is 128: there the bound is 1056 KB (32 / 8 x 128, prefix of 4096: 16 rows,
-// 1056 KB, 28 us against 40 us; prefix of 1024: 64 rows, 1024 KB, 43 us against 41 us; 32 / 4 x 64, prefix of 4096,
-// 64 rows, 950 KB: 42 us against 32 us).
+// against 29 us; but never where a sequence has at most 128 KB of codes a head, nor from 8 small CTAs an SM on, for
+// the split form's second launch then costs more than its larger rings gain (32 / 8 x 128, b 64: at 512 keys the same,
+// at 1024 keys 36 us against 29 us split; b 256: at 512 keys 55 us against 65 us, at 1024 keys 96 us against 109 us;
+// 32 / 4 x 64, b 256: at 1024 keys 37 us against 44 us, at 1536 keys, where no three fit, 69 us against 56 us).
+// Behind a shared prefix, which L2 holds, the other form is attn_kv8_tc.cu, whose five launches take 30 to 40 us at
+// least where head_dim is 128: there the bound is 1056 KB (32 / 8 x 128, prefix of 4096: 16 rows, 1056 KB, 28 us
+// against 40 us; prefix of 1024: 64 rows, 1024 KB, 32 us against 41 us; 32 / 4 x 64, prefix of 4096, 64 rows, 950 KB:
+// 42 us against 32 us).
 struct ClusterPlan {
-  int size, cap;
+  int size, cap, warps;
   size_t smem;
 };
 
 template <int HD, int GP>
 int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan) {
-  using M = ClusterSmem<HD, GP>;
-  auto kern = decode_kv8_kernel<HD, GP>;
+  using M = ClusterSmem<HD, GP, 8>;
+  auto kern = decode_kv8_kernel<HD, GP, 8>;
   // clusters of 1, 2, 4, 8, 16 CTAs resident at once, by CTAs of all the shared memory and of what fits twice
   static int resident[64][2][5] = {};
   static size_t twice[64] = {};
@@ -847,7 +860,7 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
       for (int i = 0; i < 5; ++i) {
         cudaLaunchAttribute attr[2];
         const size_t smem = half ? twice[device] : SMEM_MAX;
-        cudaLaunchConfig_t probe = launch_config(dim3(1 << i), DT, smem, nullptr, 1 << i, attr);
+        cudaLaunchConfig_t probe = launch_config(dim3(1 << i), 256, smem, nullptr, 1 << i, attr);
         int fit = 0;
         if (cudaOccupancyMaxActiveClusters(&fit, (const void*)kern, &probe) != cudaSuccess) {
           cudaGetLastError();
@@ -859,6 +872,8 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
   }
   const int64_t bg = (int64_t)B * a.c.n_kv;
   const int64_t blocks = ((int64_t)a.prefix_len + 31) / 32 + ((int64_t)a.max_len + 31) / 32, keys = 32 * blocks;
+  constexpr int AN_SM = ctas_by_registers<HD, GP>(8);
+  const size_t smem4 = ClusterSmem<HD, GP, 4>::bytes(keys);
   plan = {};
   for (int i = 4; i >= 0; --i) {
     const int cl = 1 << i;
@@ -870,7 +885,10 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
     if (smem > SMEM_MAX || (cl > 1 && bg > fit)) continue;
     const int64_t codes = keys * 2 * HD, ctas = bg * cl;
     const int64_t most = a.prefix_len > 0 && HD == 128 ? 1056 * 1024 : 600 * 1024;
-    if (codes <= 128 * 1024 || bg * codes / (ctas < sms ? ctas : sms) <= most) plan = {cl, (int)cap, smem};
+    const bool small = cl == 1 && bg > (int64_t)AN_SM * sms && smem4 <= (AN_SM == 2 ? 74 : 112) * 1024;
+    const bool waves = small && bg >= 8ll * sms && a.prefix_len == 0;
+    if (codes <= 128 * 1024 || bg * codes / (ctas < sms ? ctas : sms) <= most || waves)
+      plan = {cl, (int)cap, small ? 4 : 8, small ? smem4 : smem};
     break;
   }
   return SM_OK;
@@ -879,30 +897,35 @@ int plan_cluster(const Kv8Attn& a, int B, int device, int sms, ClusterPlan& plan
 template <int HD, int GP>
 int launch_decode_cluster(const Kv8Attn& a, const Kv8Behind& o, int B, const ClusterPlan& plan, cudaStream_t st) {
   cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = launch_config(dim3(plan.size, a.c.n_kv, B), DT, plan.smem, st, plan.size, attr);
-  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, decode_kv8_kernel<HD, GP>, a, o, plan.cap));
+  auto kern = plan.warps == 4 ? decode_kv8_kernel<HD, GP, 4> : decode_kv8_kernel<HD, GP, 8>;
+  if (plan.warps == 4)
+    SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_MAX));
+  const cudaLaunchConfig_t cfg =
+      launch_config(dim3(plan.size, a.c.n_kv, B), 32 * plan.warps, plan.smem, st, plan.size, attr);
+  SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, a, o, plan.cap));
   return SM_OK;
 }
 
-template <int HD, int GP>
+template <int HD, int GP, int W>
 int launch_split_kernel(const Kv8Split& s, int B, bool pv, cudaStream_t st) {
-  auto kern = pv ? split_pv_kernel<HD, GP> : split_scores_kernel<HD, GP>;
-  const int smem = pv ? SplitSmem<HD, GP, true>::RING : SplitSmem<HD, GP, false>::RING;
+  auto kern = pv ? split_pv_kernel<HD, GP, W> : split_scores_kernel<HD, GP, W>;
+  const int smem = pv ? SplitSmem<HD, GP, W, true>::RING : SplitSmem<HD, GP, W, false>::RING;
   SM_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   cudaLaunchAttribute attr[2];
-  const cudaLaunchConfig_t cfg = launch_config(dim3(s.n_chunks, s.a.c.n_kv, B), DT, smem, st, 1, attr);
+  const cudaLaunchConfig_t cfg = launch_config(dim3(s.n_chunks, s.a.c.n_kv, B), 32 * W, smem, st, 1, attr);
   SM_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, s));
   return SM_OK;
 }
 
+template <int W>
 int launch_split_as(const Kv8Split& s, int hd, int B, bool pv, cudaStream_t st) {
   if (hd == 64)
-    return s.gp == 4   ? launch_split_kernel<64, 4>(s, B, pv, st)
-           : s.gp == 8 ? launch_split_kernel<64, 8>(s, B, pv, st)
-                       : launch_split_kernel<64, 16>(s, B, pv, st);
-  return s.gp == 4   ? launch_split_kernel<128, 4>(s, B, pv, st)
-         : s.gp == 8 ? launch_split_kernel<128, 8>(s, B, pv, st)
-                     : launch_split_kernel<128, 16>(s, B, pv, st);
+    return s.gp == 4   ? launch_split_kernel<64, 4, W>(s, B, pv, st)
+           : s.gp == 8 ? launch_split_kernel<64, 8, W>(s, B, pv, st)
+                       : launch_split_kernel<64, 16, W>(s, B, pv, st);
+  return s.gp == 4   ? launch_split_kernel<128, 4, W>(s, B, pv, st)
+         : s.gp == 8 ? launch_split_kernel<128, 8, W>(s, B, pv, st)
+                     : launch_split_kernel<128, 16, W>(s, B, pv, st);
 }
 
 // Sizes the split form and returns the floats that its arrays take together.
@@ -915,6 +938,9 @@ int64_t plan_split(Kv8Split& s, int hd, int B, int sms) {
   // 3552 54 us; b 64, 4096 to 8192 keys: of 1024 193 us, of 2048 159 us, of 4096 154 us)
   const int ctas = s.gp == 4 || (hd == 64 && s.gp == 8) ? 2 : 1;
   const int64_t wave = std::max<int64_t>(1, (int64_t)ctas * sms / bg);
+  // 4 warps a CTA where there are waves of single chunks (32 / 8 x 128: b 64, 1024 keys 29 us against 36 us, b 256, 512
+  // to 2048 keys 128 us against 141 us; longer ones the same time, and few sequences 57 us against 54 us)
+  s.warps = wave == 1 && s.a.max_len <= 4096 ? 4 : 8;
   s.chunk = (int)std::min<int64_t>(4096, std::max<int64_t>(512, ((s.a.max_len + wave - 1) / wave + 31) & ~31LL));
   s.n_chunks = ceil_div(s.a.max_len, s.chunk);
   const int64_t rows = bg * s.n_chunks;
@@ -928,8 +954,9 @@ int launch_split(Kv8Split& s, float* base, int hd, int B, cudaStream_t st) {
   s.stat = s.pacc + rows * s.gp * hd;
   s.unit = s.stat + rows * (2 * s.gp + 1);
   s.arrived = (int*)(s.unit + (int64_t)B * s.a.c.n_kv * s.gp);
-  SM_TRY(launch_split_as(s, hd, B, false, st));
-  return launch_split_as(s, hd, B, true, st);
+  for (bool pv : {false, true})
+    SM_TRY(s.warps == 4 ? launch_split_as<4>(s, hd, B, pv, st) : launch_split_as<8>(s, hd, B, pv, st));
+  return SM_OK;
 }
 
 int launch_decode_split(const Kv8Attn& a, int hd, int B, int sms, cudaStream_t st) {
@@ -1016,6 +1043,7 @@ int plan_kv8_own(Kv8Own& own, int hd, int B, int device, int sms) {
                            [&](auto form) { return form.plan(own.a, B, device, sms, plan); }));
   own.cluster = plan.size;
   own.cap = plan.cap;
+  own.warps = plan.warps;
   own.smem = plan.smem;
   Kv8Split s = {};
   s.a = own.a;
@@ -1027,7 +1055,7 @@ int launch_kv8_own(const Kv8Own& own, float* workspace, int hd, int B, int sms, 
   if (own.cluster) {
     ++*n_launch;
     return with_cluster_form(hd, own.a.n_heads / own.a.c.n_kv, [&](auto form) {
-      return form.launch(own.a, own.behind, B, ClusterPlan{own.cluster, own.cap, own.smem}, st);
+      return form.launch(own.a, own.behind, B, ClusterPlan{own.cluster, own.cap, own.warps, own.smem}, st);
     });
   }
   *n_launch += 2;

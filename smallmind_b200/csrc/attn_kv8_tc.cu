@@ -22,7 +22,7 @@
 // Bound by the tensor cores: at fp32 accuracy a block takes 16 + 32 MMAs (head_dim 128) in the two passes, 64 clocks
 // each.  32 / 8 heads of 128, 256 rows over 32768 keys: max 95 us (82% of the time on the tensor pipe), P V 218 us
 // (72%: P of a block is waited for while both score buffers are taken), prep 33 us (HBM: 67 MB of codes in, 134 MB
-// of tiles out), own keys 67 us, join 10 us.  Four score buffers of 64 keys keep the pipe full, but an MMA of 64
+// of tiles out), own keys 45 us, join 10 us.  Four score buffers of 64 keys keep the pipe full, but an MMA of 64
 // columns takes as long as one of 128 (P V 238 us); two halves of the softmax warps that take every other block
 // 230 us; 8 softmax warps instead of 16 the same time.
 #include <cuda_fp16.h>

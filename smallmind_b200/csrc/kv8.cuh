@@ -93,7 +93,7 @@ struct Kv8Behind {
 struct Kv8Own {
   Kv8Attn a;                 // prefix_len 0
   Kv8Behind behind;
-  int cluster, cap;          // the cluster form's size and keys of a CTA; 0: the split form
+  int cluster, cap, warps;   // the cluster form's size, keys and warps of a CTA; 0: the split form
   size_t smem;
   int64_t floats;            // the split form's workspace
 };

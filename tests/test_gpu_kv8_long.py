@@ -58,6 +58,31 @@ def test_large_batches_on_both_sides_of_the_split(ctx, n_heads, n_kv, hd, B, lon
     assert ctx.device_status() == 0
 
 
+@pytest.mark.parametrize("n_heads,n_kv,hd,B,longest", [
+    (16, 2, 128, 160, 600), (16, 1, 128, 600, 1000), (32, 4, 128, 150, 1100), (16, 1, 64, 900, 1500),
+    (12, 4, 64, 400, 1200), (16, 1, 64, 320, 200), (7, 7, 128, 90, 100), (4, 4, 64, 120, 4097), (4, 4, 64, 120, 4000)])
+def test_many_rows(ctx, n_heads, n_kv, hd, B, longest):
+    """More sequences than fit the GPU at once, at every group size of both forms."""
+    rs = np.random.RandomState(B + longest)
+    lens = rs.randint(0, longest + 1, B)
+    lens[:3] = longest, 0, longest - 1
+    seq = rs.permutation(B)
+    held = np.zeros(B, int)
+    held[seq] = lens
+    seq[4] = -1
+    c = Cache(ctx, B, longest, n_kv, hd).fill(rs, held)
+    c.vs[seq[2], n_kv - 1, lens[2]:] = float("inf")  # behind the length: not seen
+    q = (rs.randn(B, n_heads, hd) * np.exp(rs.randn(B, n_heads, 1))).astype(np.float32)
+    a = c.arrays()
+    some = np.unique(np.r_[:6, B - 2:B, rs.randint(0, B, 24)])
+    keys = [None if seq[b] < 0 else [(a, seq[b], lens[b])] for b in some]
+    got = run_decode(ctx, c, q, seq, lens, longest, q_stride=n_heads * hd + 1)
+    check(got[some], *kv8_ref.attend_rows(q[some], n_kv, keys))
+    assert (got[4] == 5.0).all() and not got[1].any() and np.isfinite(got).all()
+    assert np.array_equal(got, run_decode(ctx, c, q, seq, lens, longest))
+    assert ctx.device_status() == 0
+
+
 @pytest.mark.parametrize("n_heads,n_kv,hd,B,prefix_len,longest", [
     (32, 8, 128, 64, 1500, 1100), (16, 2, 64, 180, 1301, 1600), (16, 1, 64, 330, 900, 1300), (4, 4, 128, 140, 640, 800)])
 def test_long_own_keys_behind_a_shared_prefix(ctx, n_heads, n_kv, hd, B, prefix_len, longest):
