@@ -29,9 +29,8 @@ namespace {
 //           the warp's keys, in the registers that the MMA wants them in; V codes are made
 //           fragments by 4 x 4 byte transposes.  With up to 4 heads the three digits of all of
 //           them are rows of one A operand; with more, a digit is a B operand of 8 heads.
-// The kernels come with W = 8 and with W = 4 warps a CTA: twice as many of the smaller CTAs hide one another's phases
-// better once there are more of them than an SM holds.
-
+// The kernels come with W = 8 and with W = 4 warps a CTA: the smaller CTAs, twice as many on an SM, hide one
+// another's phases better once there are waves of them.
 template <int HD, int GP>
 struct Tile {
   static constexpr bool PA = GP == 4;           // P's digits as the A operand

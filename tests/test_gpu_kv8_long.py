@@ -284,3 +284,47 @@ def test_magnitudes(ctx, B, n, P, k_size, v_size, q_size):
     want, tol = kv8_ref.attend_rows(q[some], n_kv, keys)
     check(got[some], want, tol + 64 * 2.0 ** -150)
     assert np.isfinite(got).all() and got.any()
+
+
+def test_two_host_threads():
+    """Calls of every form from two host threads at once, each with its own context and stream."""
+    import threading
+
+    import torch
+
+    import smallmind_b200 as sm
+    n_heads, n_kv, hd, T, P = 16, 4, 64, 1300, 700
+    failures = []
+
+    def work(seed):
+        try:
+            rs = np.random.RandomState(seed)
+            ctx = sm.CudaContext(0)
+            s = torch.cuda.Stream()
+            ctx.set_stream(s.cuda_stream)
+            for B in (3, 90, 160):
+                lens = rs.randint(0, T + 1, B)
+                with torch.cuda.stream(s):
+                    c = Cache(ctx, B, T, n_kv, hd).fill(rs, lens)
+                    p = Cache(ctx, 1, P, n_kv, hd).fill(rs, [P])
+                    q = rs.randn(B, n_heads, hd).astype(np.float32)
+                    first = [run_decode(ctx, c, q, None, lens, T), run_decode(ctx, c, q, None, lens, T, p, 0, P)]
+                    for _ in range(5):
+                        again = [run_decode(ctx, c, q, None, lens, T), run_decode(ctx, c, q, None, lens, T, p, 0, P)]
+                        assert all(np.array_equal(x, y) for x, y in zip(first, again))
+                    a, pa = c.arrays(), p.arrays()
+                some = [0, B - 1]
+                check(first[0][some], *kv8_ref.attend_rows(q[some], n_kv, [[(a, b, lens[b])] for b in some]))
+                keys = [[(pa, 0, P), (a, b, lens[b])] for b in some]
+                check(first[1][some], *kv8_ref.attend_rows(q[some], n_kv, keys))
+            assert ctx.device_status() == 0
+            ctx.close()
+        except BaseException as e:
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
