@@ -23,8 +23,8 @@ namespace {
 // Keys are taken in blocks of 32, a warp each:
 //   scores  two 16-key x 8-head MMA tiles.  K codes are A fragments as they lie: a lane takes 16
 //           neighbouring bytes of a row, and q's digits, built once, are in the matching order.  A lane's
-//           four rows are the keys whose scores the P side wants side by side.  Scores are kept without the
-//           head's positive factor, which a maximum does not need;
+//           four rows are the keys whose scores the P side wants side by side.  Scores are kept as they are
+//           compared and subtracted, so that x is 0 at the largest one, not a rounding above it;
 //   P V     weights e, and P = e * v_scale in 23-bit fixed point against the largest v_scale of
 //           the warp's keys, in the registers that the MMA wants them in; V codes are made
 //           fragments by 4 x 4 byte transposes.  With up to 4 heads the three digits of all of
@@ -98,12 +98,22 @@ struct KBlock {
   float s[4];
 };
 
-// Scores of a block: to z ([NT] planes `plane` floats apart), and this lane's running maxima of columns 2t, 2t + 1.
+// Factors of columns 2t, 2t + 1, from the lanes whose column heads they are
+template <int NT>
+__device__ __forceinline__ void column_units(const float (&unit)[NT], int t, float (&of)[NT][2]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) of[nt][i] = __shfl_sync(0xffffffffu, unit[nt], (2 * t + i) * 4);
+}
+
+// Scores of a block: to z ([NT] planes `plane` floats apart), and this lane's running maxima of columns 2t, 2t + 1,
+// whose factors are `unit`.
 template <int HD, int GP>
 __device__ __forceinline__ void score_block(const KBlock<HD>& k,
                                             const uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
-                                            int g, int t, float* z, int64_t plane,
-                                            float (&mx)[Tile<HD, GP>::NT][2]) {
+                                            const float (&unit)[Tile<HD, GP>::NT][2], int g, int t, float* z,
+                                            int64_t plane, float (&mx)[Tile<HD, GP>::NT][2]) {
   using T = Tile<HD, GP>;
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) {
@@ -121,7 +131,7 @@ __device__ __forceinline__ void score_block(const KBlock<HD>& k,
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        s[2 * m + (i >> 1)][i & 1] = join3_small(d[2][i], d[1][i], d[0][i]) * k.s[2 * m + (i >> 1)];
+        s[2 * m + (i >> 1)][i & 1] = join3_small(d[2][i], d[1][i], d[0][i]) * k.s[2 * m + (i >> 1)] * unit[nt][i & 1];
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -167,19 +177,19 @@ struct PVSum {
     return T::PA ? (g & 3) * 32 + t * 8 + (g >> 2) * 4 : g * 32 + t * 8;
   }
 
-  float m[T::NT], unit[T::NT], esum[T::NT];  // of this lane's head: maximum, factor of the scores, sum of weights
-  float top, inv;                            // largest V scale and 1 / it
+  float m[T::NT], esum[T::NT];  // of this lane's head: maximum and sum of weights
+  float top, inv;               // largest V scale and 1 / it
   int acc[T::MD][T::MT][4];
 
   // Fixed point: e = 1 at the largest scale is POINT = 2^23 - 8.  In two factors each way, so that none of them
   // leaves the normal numbers; scales below those keep their resolution.
   static constexpr float POINT = 8388600.f;
   __device__ __forceinline__ float value(float sum) const { return sum * (1.f / POINT) * top; }
-  __device__ __forceinline__ void start(float vmax, const float (&max_of)[T::NT], const float (&unit_of)[T::NT]) {
+  __device__ __forceinline__ void start(float vmax, const float (&max_of)[T::NT]) {
     top = max_nan(vmax, 0x1p-126f);
     inv = 1.f / top;
 #pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt) unit[nt] = unit_of[nt], m[nt] = max_of[nt], esum[nt] = 0.f;
+    for (int nt = 0; nt < T::NT; ++nt) m[nt] = max_of[nt], esum[nt] = 0.f;
 #pragma unroll
     for (int i = 0; i < T::MD; ++i)
 #pragma unroll
@@ -198,7 +208,7 @@ struct PVSum {
     for (int nt = 0; nt < T::NT; ++nt) {
       float e[NZ];
 #pragma unroll
-      for (int i = 0; i < NZ; ++i) e[i] = kv8_weight(fmaf(zv[nt][i], unit[nt], -m[nt]));
+      for (int i = 0; i < NZ; ++i) e[i] = kv8_weight(zv[nt][i] - m[nt]);
       if (keys < 32) {
 #pragma unroll
         for (int i = 0; i < NZ; ++i)
@@ -209,7 +219,7 @@ struct PVSum {
 #pragma unroll
       for (int i = 0; i < NZ; ++i) {
         part += e[i];
-        // e * scale lies in [0, 2^23): added to 2^23 it is the mantissa, rounded
+        // x <= 0, so e * scale lies in [0, 2^23): added to 2^23 it is the mantissa, rounded
         p[i] = __float_as_uint(fmaf(e[i], __shfl_sync(0xffffffffu, vsm, first + 4 * i), 8388608.f));
       }
       esum[nt] += part;
@@ -455,8 +465,9 @@ __global__ void __launch_bounds__(32 * W, ctas_by_registers<HD, GP>(W))
 
   float vmax = 0.f;
   uint32_t qd[T::NT][HD / 32][3][2];
-  float unit[T::NT], mx[T::NT][2];
+  float unit[T::NT], units[T::NT][2], mx[T::NT][2];
   load_q<HD, GP>(a.q + (int64_t)b * a.q_stride + (int64_t)gk * G * HD, a.q_vec, G, lane, qd, unit);
+  column_units(unit, t, units);
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
   for (int i = 0; i < nk; ++i) {
@@ -464,7 +475,7 @@ __global__ void __launch_bounds__(32 * W, ctas_by_registers<HD, GP>(W))
     KBlock<HD> k;
     S::read_k(ring + i % M::N * S::BYTES, k, vmax, lane);
     fetch(i + M::N - 1);  // into the slot of block i - 1
-    score_block<HD, GP>(k, qd, g, t, z + (warp + DW * i) * T::ZB, plane, mx);
+    score_block<HD, GP>(k, qd, units, g, t, z + (warp + DW * i) * T::ZB, plane, mx);
   }
   warp_maxima<HD, GP>(mx, g, t, wred[warp]);
   vmax = warp_max_nan(vmax);
@@ -491,15 +502,14 @@ __global__ void __launch_bounds__(32 * W, ctas_by_registers<HD, GP>(W))
   float max_of[T::NT];
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) {
-    unit[nt] = __shfl_sync(0xffffffffu, unit[nt], col * 4);
-    max_of[nt] = gmax[nt * 8 + col] * unit[nt];
+    max_of[nt] = gmax[nt * 8 + col];
     const int h = nt * 8 + col;
     if (o.prefix_max && h < G) {
       if (rank == 0 && warp == 0 && t == 0 && g == col) o.own_max[row0 + h] = max_of[nt];
       max_of[nt] = fmaxf(max_of[nt], o.prefix_max[row0 + h] * o.prefix_unit[row0 + h]);
     }
   }
-  pv.start(vmax, max_of, unit);
+  pv.start(vmax, max_of);
   for (int i = nk; i < nk + nv; ++i) {
     const int blk = tw + TW * (i - nk);
     cp_wait<M::N - 2>();
@@ -568,7 +578,6 @@ struct Kv8Split {
   float* z;             // [B][n_kv][gp / 8 or 1][blocks] blocks of scores
   float* pacc;          // [B][n_kv][n_chunks][gp][head_dim]
   float* stat;          // [B][n_kv][n_chunks][2 * gp + 1] maxima, largest V scale; then the weights' sums
-  float* unit;          // [B][n_kv][gp] factors of the heads' scores
   int* arrived;         // [B][n_kv] chunks whose P V is done
 };
 
@@ -594,7 +603,7 @@ __global__ void __launch_bounds__(32 * W, (SplitSmem<HD, GP, W, false>::CTAS)) s
   const int G = a.n_heads / a.c.n_kv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float wred[DW][GP], vred[DW], unit_of[GP];
+  __shared__ float wred[DW][GP], vred[DW];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // only now: what the next kernel reads before its own wait has then been written
   asm volatile("griddepcontrol.launch_dependents;");
@@ -622,8 +631,9 @@ __global__ void __launch_bounds__(32 * W, (SplitSmem<HD, GP, W, false>::CTAS)) s
   for (int i = 0; i < M::N - 1; ++i) fetch(32 * (warp + DW * i), i);
   float vmax = 0.f;
   uint32_t qd[T::NT][HD / 32][3][2];
-  float unit[T::NT], mx[T::NT][2];
+  float unit[T::NT], units[T::NT][2], mx[T::NT][2];
   load_q<HD, GP>(a.q + (int64_t)b * a.q_stride + (int64_t)gk * G * HD, a.q_vec, G, lane, qd, unit);
+  column_units(unit, t, units);
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) mx[nt][0] = mx[nt][1] = -INFINITY;
   int at = 0;
@@ -634,17 +644,12 @@ __global__ void __launch_bounds__(32 * W, (SplitSmem<HD, GP, W, false>::CTAS)) s
     // the slot of the block before this one is free
     fetch(row + 32 * DW * (M::N - 1), at == 0 ? M::N - 1 : at - 1);
     at = at == M::N - 1 ? 0 : at + 1;
-    score_block<HD, GP>(k, qd, g, t, z + (int64_t)(row >> 5) * T::ZB, plane, mx);
+    score_block<HD, GP>(k, qd, units, g, t, z + (int64_t)(row >> 5) * T::ZB, plane, mx);
   }
   cp_wait<0>();
   warp_maxima<HD, GP>(mx, g, t, wred[warp]);
   vmax = warp_max_nan(vmax);
   if (lane == 0) vred[warp] = vmax;
-  if (warp == 0 && t == 0) {
-#pragma unroll
-    for (int nt = 0; nt < T::NT; ++nt)
-      if (g < T::CP) unit_of[nt * 8 + g] = unit[nt];
-  }
   __syncthreads();
   float* stat = s.stat + (bg * s.n_chunks + ch) * (2 * GP + 1);
   if (tid < GP) {
@@ -652,9 +657,8 @@ __global__ void __launch_bounds__(32 * W, (SplitSmem<HD, GP, W, false>::CTAS)) s
 #pragma unroll
     for (int i = 0; i < DW; ++i) m = fmaxf(m, wred[i][tid]);
     stat[tid] = m;
-    if (ch == 0) s.unit[bg * GP + tid] = unit_of[tid];
     if (s.o.prefix_max && tid < G)
-      atomic_max(s.o.own_max + (int64_t)gk * s.o.rows + (int64_t)b * G + tid, m * unit_of[tid]);
+      atomic_max(s.o.own_max + (int64_t)gk * s.o.rows + (int64_t)b * G + tid, m);
   } else if (tid == GP) {
 #pragma unroll
     for (int i = 0; i < DW; ++i) vmax = max_nan(vmax, vred[i]);
@@ -712,7 +716,7 @@ __global__ void __launch_bounds__(32 * W, (SplitSmem<HD, GP, W, true>::CTAS)) sp
   const int col = pv.column(g);
   float* stat = s.stat + bg * s.n_chunks * (2 * GP + 1);
   const int used = (len + s.chunk - 1) / s.chunk;
-  float max_of[T::NT], unit[T::NT];
+  float max_of[T::NT];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
 #pragma unroll
@@ -727,21 +731,18 @@ __global__ void __launch_bounds__(32 * W, (SplitSmem<HD, GP, W, true>::CTAS)) sp
     gmax[warp][lane] = m;
   }
   const float vmax = stat[ch * (2 * GP + 1) + GP];
-#pragma unroll
-  for (int nt = 0; nt < T::NT; ++nt) unit[nt] = s.unit[bg * GP + nt * 8 + col];
   __syncthreads();
 #pragma unroll
   for (int nt = 0; nt < T::NT; ++nt) {
     max_of[nt] = -INFINITY;
 #pragma unroll
     for (int i = 0; i < DW; ++i) max_of[nt] = fmaxf(max_of[nt], gmax[i][nt * 8 + col]);
-    max_of[nt] *= unit[nt];
     if (s.o.prefix_max && nt * 8 + col < G) {
       const int64_t row = row0 + nt * 8 + col;
       max_of[nt] = fmaxf(max_of[nt], s.o.prefix_max[row] * s.o.prefix_unit[row]);
     }
   }
-  pv.start(vmax, max_of, unit);
+  pv.start(vmax, max_of);
   int at = 0;
   for (int row = 32 * tw; row < n; row += 32 * TW) {
     cp_wait<M::N - 2>();
@@ -943,7 +944,7 @@ int64_t plan_split(Kv8Split& s, int hd, int B, int sms) {
   s.chunk = (int)std::min<int64_t>(4096, std::max<int64_t>(512, ((s.a.max_len + wave - 1) / wave + 31) & ~31LL));
   s.n_chunks = ceil_div(s.a.max_len, s.chunk);
   const int64_t rows = bg * s.n_chunks;
-  return rows * s.chunk * s.gp + rows * s.gp * hd + rows * (2 * s.gp + 1) + bg * s.gp + bg;
+  return rows * s.chunk * s.gp + rows * s.gp * hd + rows * (2 * s.gp + 1) + bg;
 }
 
 int launch_split(Kv8Split& s, float* base, int hd, int B, cudaStream_t st) {
@@ -951,8 +952,7 @@ int launch_split(Kv8Split& s, float* base, int hd, int B, cudaStream_t st) {
   s.z = base;
   s.pacc = s.z + rows * s.chunk * s.gp;
   s.stat = s.pacc + rows * s.gp * hd;
-  s.unit = s.stat + rows * (2 * s.gp + 1);
-  s.arrived = (int*)(s.unit + (int64_t)B * s.a.c.n_kv * s.gp);
+  s.arrived = (int*)(s.stat + rows * (2 * s.gp + 1));
   for (bool pv : {false, true})
     SM_TRY(s.warps == 4 ? launch_split_as<4>(s, hd, B, pv, st) : launch_split_as<8>(s, hd, B, pv, st));
   return SM_OK;

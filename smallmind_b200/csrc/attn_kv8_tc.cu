@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
         // the row's maximum over the prefix and the own keys
         const float unit = s.unit[row];
         const float m = fmaxf(s.row_max[row] * unit, s.own_max[row]);
-        const Pair unit2(unit), minus_m(-m);
+        const Pair unit2(unit);
         Pair sum2(0.f);
         // weights of 16 keys, P over their scores; TAIL: only the first `left` keys exist
         auto weigh = [&](auto tail, uint32_t cols, const uint32_t (&x)[16], uint32_t k4, int left) {
@@ -538,7 +538,11 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
             for (int o = 0; o < 2; ++o) {
               const Pair t = mul2(Pair(__uint_as_float(x[e + 2 * o]), __uint_as_float(x[e + 2 * o + 1])),
                                   o ? Pair(k.z, k.w) : Pair(k.x, k.y));
-              Pair w = kv8_weight2(fma2(t, unit2, minus_m));
+              // m is the largest of these rounded products, so the difference is 0 there and nowhere above: it must
+              // not become one FMA with the product, as the packed add and multiply do (seen in their results)
+              float z0, z1;
+              mul2(t, unit2).get(z0, z1);
+              Pair w = kv8_weight2(Pair(__fsub_rn(z0, m), __fsub_rn(z1, m)));
               if constexpr (TAIL) {
                 float w0, w1;
                 w.get(w0, w1);
