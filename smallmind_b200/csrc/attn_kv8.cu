@@ -108,7 +108,8 @@ __device__ __forceinline__ void column_units(const float (&unit)[NT], int t, flo
 }
 
 // Scores of a block: to z ([NT] planes `plane` floats apart), and this lane's running maxima of columns 2t, 2t + 1,
-// whose factors are `unit`.
+// whose factors are `unit`.  The factors meet first: a sum of up to 2^36 times a large scale would leave fp32's range
+// where the score does not.
 template <int HD, int GP>
 __device__ __forceinline__ void score_block(const KBlock<HD>& k,
                                             const uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
@@ -131,7 +132,7 @@ __device__ __forceinline__ void score_block(const KBlock<HD>& k,
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        s[2 * m + (i >> 1)][i & 1] = join3_small(d[2][i], d[1][i], d[0][i]) * k.s[2 * m + (i >> 1)] * unit[nt][i & 1];
+        s[2 * m + (i >> 1)][i & 1] = join3_small(d[2][i], d[1][i], d[0][i]) * (k.s[2 * m + (i >> 1)] * unit[nt][i & 1]);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -506,7 +507,7 @@ __global__ void __launch_bounds__(32 * W, ctas_by_registers<HD, GP>(W))
     const int h = nt * 8 + col;
     if (o.prefix_max && h < G) {
       if (rank == 0 && warp == 0 && t == 0 && g == col) o.own_max[row0 + h] = max_of[nt];
-      max_of[nt] = fmaxf(max_of[nt], o.prefix_max[row0 + h] * o.prefix_unit[row0 + h]);
+      max_of[nt] = fmaxf(max_of[nt], o.prefix_max[row0 + h]);
     }
   }
   pv.start(vmax, max_of);
@@ -737,10 +738,7 @@ __global__ void __launch_bounds__(32 * W, (SplitSmem<HD, GP, W, true>::CTAS)) sp
     max_of[nt] = -INFINITY;
 #pragma unroll
     for (int i = 0; i < DW; ++i) max_of[nt] = fmaxf(max_of[nt], gmax[i][nt * 8 + col]);
-    if (s.o.prefix_max && nt * 8 + col < G) {
-      const int64_t row = row0 + nt * 8 + col;
-      max_of[nt] = fmaxf(max_of[nt], s.o.prefix_max[row] * s.o.prefix_unit[row]);
-    }
+    if (s.o.prefix_max && nt * 8 + col < G) max_of[nt] = fmaxf(max_of[nt], s.o.prefix_max[row0 + nt * 8 + col]);
   }
   pv.start(vmax, max_of);
   int at = 0;

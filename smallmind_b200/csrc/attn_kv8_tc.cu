@@ -5,7 +5,8 @@
 // maximum over the prefix and the own keys comes first, so the scores are formed twice:
 //   prep    K and V codes -> fp16 tiles (codes are exact in fp16), query rows, scaled by a power of two into
 //           [-1, 1], -> fp16 pairs hi + lo (22 bits);
-//   max     S = (hi + lo) K^T per tile of 128 rows and block of 128 keys; row maxima of S * k_scale;
+//   max     S = (hi + lo) K^T per tile of 128 rows and block of 128 keys; row maxima of the scores S * (k_scale *
+//           the row's factor): the factors meet first, or S times a large scale would leave fp32's range;
 //   own     (attn_kv8.cu) the sequences' own keys, against the maximum of both parts;
 //   P V     S again, e against the maximum of both parts, P = e * v_scale relative to the prefix's largest
 //           scale as fp16 pairs hi + lo, O += (hi + lo) V;
@@ -62,7 +63,7 @@ struct SharedArgs {
   float* scales;            // [n_kv][n_blocks][K 128 | V 128]; past the prefix NaN | 0
   uint8_t* qt;              // [n_kv][tiles][hi | lo][128 rows][HD] fp16
   float* unit;              // [n_kv][tiles * 128] factor of a row's scores
-  float* row_max;           // [n_kv][tiles * 128] largest S * k_scale
+  float* row_max;           // [n_kv][tiles * 128] largest score over the prefix
   float* v_max;             // [n_kv][n_blocks][4] largest V scales of 32 keys each
   float* v_top;             // [n_kv] the head's largest, at least 2^-126
   float* acc;               // [segment][128][HD]; segment = CTA + tile of all kv heads, in lines (segment_of)
@@ -303,7 +304,7 @@ struct Ring {
   }
 };
 
-// MAX: row maxima of S * k_scale, and the V scales relative to their largest.  Else: the segments' O and weight sums.
+// MAX: row maxima of the scores, and the V scales relative to their largest.  Else: the segments' O and weight sums.
 template <int HD, bool MAX>
 __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_constant__ SharedArgs s) {
   using M = TcSmem<HD, MAX>;
@@ -489,6 +490,7 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
       }
       if constexpr (MAX) {
         float m = -INFINITY;
+        const Pair unit2(s.unit[row]);
         for (int i = 0; i < nb; ++i) {
           enter();
           const uint32_t k4 = smem_u32(smem + M::SCALES + sc.slot * (2 * KB * 4)) + part * (PK * 4);
@@ -505,8 +507,10 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
             for (int e = 0; e < 32; e += 4) {
               const float4 k = ld_slot(k4 + (32 * c + e) * 4);
               float y[4];
-              mul2(Pair(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])), Pair(k.x, k.y)).get(y[0], y[1]);
-              mul2(Pair(__uint_as_float(x[c][e + 2]), __uint_as_float(x[c][e + 3])), Pair(k.z, k.w)).get(y[2], y[3]);
+              mul2(Pair(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])), mul2(Pair(k.x, k.y), unit2))
+                  .get(y[0], y[1]);
+              mul2(Pair(__uint_as_float(x[c][e + 2]), __uint_as_float(x[c][e + 3])), mul2(Pair(k.z, k.w), unit2))
+                  .get(y[2], y[3]);
               m = fmaxf(fmaxf(m, fmaxf(y[0], y[1])), fmaxf(y[2], y[3]));
             }
           arrive(&sc_free[sc.slot]);
@@ -523,9 +527,8 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
         soft_sync();
       } else {
         // the row's maximum over the prefix and the own keys
-        const float unit = s.unit[row];
-        const float m = fmaxf(s.row_max[row] * unit, s.own_max[row]);
-        const Pair unit2(unit);
+        const float m = fmaxf(s.row_max[row], s.own_max[row]);
+        const Pair unit2(s.unit[row]);
         Pair sum2(0.f);
         // weights of 16 keys, P over their scores; TAIL: only the first `left` keys exist
         auto weigh = [&](auto tail, uint32_t cols, const uint32_t (&x)[16], uint32_t k4, int left) {
@@ -536,12 +539,11 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
             const float4 k = ld_slot(k4 + 4 * e), v = ld_slot(k4 + 4 * (KB + e));
 #pragma unroll
             for (int o = 0; o < 2; ++o) {
-              const Pair t = mul2(Pair(__uint_as_float(x[e + 2 * o]), __uint_as_float(x[e + 2 * o + 1])),
-                                  o ? Pair(k.z, k.w) : Pair(k.x, k.y));
+              const Pair ku = mul2(o ? Pair(k.z, k.w) : Pair(k.x, k.y), unit2);
               // m is the largest of these rounded products, so the difference is 0 there and nowhere above: it must
               // not become one FMA with the product, as the packed add and multiply do (seen in their results)
               float z0, z1;
-              mul2(t, unit2).get(z0, z1);
+              mul2(Pair(__uint_as_float(x[e + 2 * o]), __uint_as_float(x[e + 2 * o + 1])), ku).get(z0, z1);
               Pair w = kv8_weight2(Pair(__fsub_rn(z0, m), __fsub_rn(z1, m)));
               if constexpr (TAIL) {
                 float w0, w1;
@@ -757,7 +759,7 @@ int launch_attention_shared_tc(const Kv8Attn& a, int hd, int B, int device, int 
     s.own_sum = s.own_acc + rp * hd;
     own_space = s.own_sum + rp;
   }
-  own.behind = {s.row_max, s.unit, s.tiles * QB, s.own_max, s.own_acc, s.own_sum};
+  own.behind = {s.row_max, s.tiles * QB, s.own_max, s.own_acc, s.own_sum};
   const int rc = hd == 64 ? launch_shared<64>(s, own, own_space, B, sms, st, n_launch)
                           : launch_shared<128>(s, own, own_space, B, sms, st, n_launch);
   cudaFreeAsync(buf, st);

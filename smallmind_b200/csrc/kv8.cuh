@@ -81,12 +81,11 @@ __device__ __forceinline__ bool row_in_range(const Kv8Attn& a, int b) {
 // For the own keys of a batch behind a shared prefix (attn_kv8_tc.cu), row = kv head * rows + b * group + head:
 // what is known of the prefix's scores, and where the own part goes.
 struct Kv8Behind {
-  const float* prefix_max;   // nullptr: there is no such prefix
-  const float* prefix_unit;  // a row's largest score is prefix_max * prefix_unit
+  const float* prefix_max;  // largest score over the prefix; nullptr: there is no such prefix
   int rows;
-  float* own_max;            // largest own score, -inf at first
-  float* acc;                // [row][head_dim] sum of weights times values
-  float* sum;                // [row] sum of weights
+  float* own_max;           // largest own score, -inf at first
+  float* acc;               // [row][head_dim] sum of weights times values
+  float* sum;               // [row] sum of weights
 };
 
 // Own-key attention behind a prefix: one launch or two; what they need beside the caller's arrays.
