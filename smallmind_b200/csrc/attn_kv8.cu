@@ -50,8 +50,8 @@ struct Tile {
 __device__ __forceinline__ int krow(int g) { return (g & 3) + 16 * (g >> 2); }
 __device__ __forceinline__ int zpos(int head, int g) { return head * 32 + (g & 3) * 8 + (g >> 2) * 4; }
 
-// q of one kv head's group as digits in B-fragment order; `unit` gets 2^(e - 22) / sqrt(HD) of this
-// lane's column head (lane / 4), the factor of its digit sums (NaN where q is not finite).
+// q of one kv head's group as digits in B-fragment order; `unit` gets 2^e / sqrt(HD) of this lane's
+// column head (lane / 4), the factor of its digit sums (NaN where q is not finite).
 template <int HD, int GP>
 __device__ __forceinline__ void load_q(const float* q, bool vec, int G, int lane,
                                        uint32_t (&qd)[Tile<HD, GP>::NT][HD / 32][3][2],
@@ -76,16 +76,16 @@ __device__ __forceinline__ void load_q(const float* q, bool vec, int G, int lane
     peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
     peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
     const bool ok = peak < INFINITY;
-    const int e = ok ? block_exp(peak) : 0;
-    const float mult = pow2i(22 - e);
-    unit[nt] = ok ? pow2i(e - 22) * (HD == 64 ? 0.125f : 0.0883883476f) : NAN;
+    const int e = ok ? query_exp(peak) : 0;
+    const Scale2 up(22 - e);
+    unit[nt] = ok ? query_unit<HD>(e) : NAN;
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const float* xs = x + 8 * i + 4 * half;
-        bytes3((uint32_t)__float2int_rn(xs[0] * mult), (uint32_t)__float2int_rn(xs[1] * mult),
-               (uint32_t)__float2int_rn(xs[2] * mult), (uint32_t)__float2int_rn(xs[3] * mult), qd[nt][i][0][half],
+        bytes3((uint32_t)__float2int_rn(up(xs[0])), (uint32_t)__float2int_rn(up(xs[1])),
+               (uint32_t)__float2int_rn(up(xs[2])), (uint32_t)__float2int_rn(up(xs[3])), qd[nt][i][0][half],
                qd[nt][i][1][half], qd[nt][i][2][half]);
       }
   }
@@ -108,7 +108,7 @@ __device__ __forceinline__ void column_units(const float (&unit)[NT], int t, flo
 }
 
 // Scores of a block: to z ([NT] planes `plane` floats apart), and this lane's running maxima of columns 2t, 2t + 1,
-// whose factors are `unit`.  The factors meet first: a sum of up to 2^36 times a large scale would leave fp32's range
+// whose factors are `unit`.  The factors meet first: a sum of up to 2^14 times a large scale would leave fp32's range
 // where the score does not.
 template <int HD, int GP>
 __device__ __forceinline__ void score_block(const KBlock<HD>& k,
@@ -132,7 +132,7 @@ __device__ __forceinline__ void score_block(const KBlock<HD>& k,
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        s[2 * m + (i >> 1)][i & 1] = join3_small(d[2][i], d[1][i], d[0][i]) * (k.s[2 * m + (i >> 1)] * unit[nt][i & 1]);
+        s[2 * m + (i >> 1)][i & 1] = join3_query(d[2][i], d[1][i], d[0][i]) * (k.s[2 * m + (i >> 1)] * unit[nt][i & 1]);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {

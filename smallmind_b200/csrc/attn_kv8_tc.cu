@@ -264,16 +264,16 @@ __global__ void __launch_bounds__(256) shared_prep_kernel(SharedArgs s) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, o));
     const bool ok = peak < INFINITY;
-    const int e = ok ? block_exp(peak) : 0;
-    const float mult = pow2i(22 - e);  // and 2^-22: 2^-e itself may not be a normal number
+    const int e = ok ? query_exp(peak) : 0;
+    const Scale2 to_unit(-e);
     if (lane == 0) {
-      s.unit[(int64_t)id * QB + r] = ok ? pow2i(e - 1) * (HD == 64 ? 0.25f : 0.176776695f) : NAN;
+      s.unit[(int64_t)id * QB + r] = ok ? query_unit<HD>(e) : NAN;
       s.row_max[(int64_t)id * QB + r] = -INFINITY;
       s.own_max[(int64_t)id * QB + r] = -INFINITY;
     }
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
-      const float y0 = ok ? x[i] * mult * 0x1p-22f : 0.f, y1 = ok ? x[i + 1] * mult * 0x1p-22f : 0.f;
+      const float y0 = ok ? to_unit(x[i]) : 0.f, y1 = ok ? to_unit(x[i + 1]) : 0.f;
       const uint32_t hi = pack_half(y0, y1);
       const float2 f = __half22float2(*(const __half2*)&hi);
       uint8_t* p = dst + (r * HD + E * lane + i) * 2;

@@ -53,12 +53,29 @@ __device__ __forceinline__ void transpose4(uint32_t& w0, uint32_t& w1, uint32_t&
   w3 = __byte_perm(c, d, 0x7632);
 }
 
-// hi * 2^16 + mid * 2^8 + lo of three digit sums; join3_small: |mid| and |lo| < 2^22
-__device__ __forceinline__ float join3_small(int hi, int mid, int lo) {
-  return fmaf((float)hi, 65536.f, (float)(mid * 256 + lo));
+// hi * 2^16 + mid * 2^8 + lo of three digit sums; join3_query: of a query's, |mid| and |lo| < 2^22, times 2^-22
+__device__ __forceinline__ float join3_query(int hi, int mid, int lo) {
+  return fmaf((float)hi, 0x1p-6f, (float)(mid * 256 + lo) * 0x1p-22f);
 }
 __device__ __forceinline__ float join3(int hi, int mid, int lo) {
   return fmaf((float)hi, 65536.f, fmaf((float)mid, 256.f, (float)lo));
+}
+
+// A query row's values are taken relative to 2^e, |x| < 2^e.  e stays at or above -120, where 2^e / sqrt(head_dim) is
+// still a normal number: below it they lose bits, of 2^-143 and less.
+__device__ __forceinline__ int query_exp(float peak) {
+  return peak > 0.f ? max(((__float_as_int(peak) >> 23) & 0xFF) - 126, -120) : 0;
+}
+// x * 2^n in two steps, as 2^n itself may not be a normal number
+struct Scale2 {
+  float a, b;
+  __device__ __forceinline__ explicit Scale2(int n) : a(pow2i(n / 2)), b(pow2i(n - n / 2)) {}
+  __device__ __forceinline__ float operator()(float x) const { return x * a * b; }
+};
+// 2^e / sqrt(HD)
+template <int HD>
+__device__ __forceinline__ float query_unit(int e) {
+  return pow2i(e - 1) * (HD == 64 ? 0.25f : 0.176776695f);
 }
 
 // Larger of the two, NaN if either is

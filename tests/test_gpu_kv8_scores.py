@@ -98,3 +98,25 @@ def test_large_k_scales_with_moderate_scores(ctx, B, n, P, n_kv, launches, hd):
     keys = [([(pa, 0, P)] if P else []) + [(a, b, lens[b])] for b in some]
     check(got[some], *kv8_ref.attend_rows(q[some], n_kv, keys))
     assert np.isfinite(got).all()
+
+
+@pytest.mark.parametrize("B,n,P,n_kv,launches", FORMS)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [1e31, 1e33, 1e36])
+def test_tiny_queries_and_large_keys(ctx, B, n, P, n_kv, launches, hd, size):
+    """Queries down to 2^-120 keep their digits."""
+    rs = np.random.RandomState(B + hd)
+    n_heads = 2 * n_kv
+    lens = rs.randint(n // 2, n + 1, B)
+    some = [0, 1, B - 1]
+    c = Cache(ctx, B, n, n_kv, hd).fill(rs, [m if b in some else 0 for b, m in enumerate(lens)])
+    p = Cache(ctx, 1, max(P, 1), n_kv, hd).fill(rs, [P])
+    for x in (c, p):
+        x.ks *= size
+    q = (rs.randn(B, n_heads, hd) / size).astype(np.float32)
+    before = ctx.launch_count()
+    got = run_decode(ctx, c, q, None, lens, n, prefix=p if P else None, prefix_len=P)
+    assert ctx.launch_count() == before + launches
+    a, pa = c.arrays(), p.arrays()
+    keys = [([(pa, 0, P)] if P else []) + [(a, b, lens[b])] for b in some]
+    check(got[some], *kv8_ref.attend_rows(q[some], n_kv, keys))
