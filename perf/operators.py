@@ -151,29 +151,36 @@ def prepare(case, seed):
 
 
 # ---------------------------------------------------------------- the framework's calls
-_context = None
+_contexts = {}  # one for each device and stream that work is queued on
 
 
-def _handle(s, which="", slots=None, tokens=None):
-    """The cache handle that a program makes once and keeps beside its tensors."""
-    global _context
-    import smallmind_b200 as sm
+def _handles(s):
+    """The cache handles that a program makes once and keeps beside its tensors, for the current stream."""
+    device = torch.cuda.current_device()
+    # the stream's number alone: torch.cuda.current_stream() takes 3 us to make an object of it
+    key = device, torch._C._cuda_getCurrentRawStream(device)
+    held = s.setdefault("handles", {})
+    if key not in held:
+        import smallmind_b200 as sm
 
-    if _context is None:
-        _context = sm.CudaContext(torch.cuda.current_device())
-        # torch's default stream has the number 0; as an explicit handle the legacy default stream is 1
-        _context.set_stream(torch.cuda.current_stream().cuda_stream or 1)
-    name = which + "handle"
-    if name not in s:
+        if key not in _contexts:
+            _contexts[key] = sm.CudaContext(device)
+            # torch's default stream has the number 0; as an explicit handle the legacy default stream is 1
+            _contexts[key].set_stream(key[1] or 1)
         c = s["case"]
-        s[name] = sm.KV8Cache(_context, *(s[which + w].data_ptr() for w in ("k", "v", "k_scale", "v_scale")),
-                              slots or s["slots"], tokens or s["tokens"], c["nkv"], c["hd"])
-    return s[name]
+
+        def make(which, slots, tokens):
+            at = (s[which + w].data_ptr() for w in ("k", "v", "k_scale", "v_scale"))
+            return sm.KV8Cache(_contexts[key], *at, slots, tokens, c["nkv"], c["hd"])
+
+        prefix = make("prefix_", 1, c["prefix"]) if c["op"] == "shared" else None
+        held[key] = make("", s["slots"], s["tokens"]), prefix
+    return held[key]
 
 
 def _run_own(s):
     c = s["case"]
-    h = _handle(s)
+    h, prefix = _handles(s)
     nh, nkv, hd = c["nh"], c["nkv"], c["hd"]
     if c["op"] in ("write", "read"):
         n = c["n"]
@@ -190,9 +197,8 @@ def _run_own(s):
         h.attention_decode_device(s["q"].data_ptr(), s["seq"].data_ptr(), s["lens"].data_ptr(), c["b"], nh,
                                   out.data_ptr(), max_len=s["longest"])
     else:
-        p = _handle(s, "prefix_", 1, c["prefix"])
-        h.attention_shared_device(s["q"].data_ptr(), p, 0, c["prefix"], s["seq"].data_ptr(), s["lens"].data_ptr(),
-                                  c["b"], nh, out.data_ptr(), max_len=s["longest"])
+        h.attention_shared_device(s["q"].data_ptr(), prefix, 0, c["prefix"], s["seq"].data_ptr(),
+                                  s["lens"].data_ptr(), c["b"], nh, out.data_ptr(), max_len=s["longest"])
     return out
 
 
