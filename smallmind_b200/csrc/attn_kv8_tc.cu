@@ -375,6 +375,12 @@ __global__ void __launch_bounds__(THREADS, 1) shared_pass_kernel(const __grid_co
           v.next<M::NV>();
         }
       }
+      // the tensor cores' last arrivals are in before the CTA's shared memory goes
+      const int n = u1 - u0;
+      for (int use = max(0, n - M::NK); use < n && ok; ++use) {
+        ok = mbar_wait_bounded(&k_free[use % M::NK], use / M::NK & 1, a.status);
+        if constexpr (!MAX) ok = ok && mbar_wait_bounded(&v_free[use % M::NV], use / M::NV & 1, a.status);
+      }
     }
   } else if (warp == MMA_WARP) {
     const uint64_t kd0 = sw128_desc(smem_u32(smem + M::K)), vd0 = sw128_desc_mn(smem_u32(smem + M::V));
