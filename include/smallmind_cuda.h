@@ -180,7 +180,8 @@ SM_API int sm_attention_decode_noalloc(sm_ctx* ctx, const float* q, const float*
  * be reused for any number of calls.
  *   k, v             int8  [max_seqs][n_kv][max_tokens][head_dim], 16-byte aligned
  *   k_scale, v_scale float [max_seqs][n_kv][max_tokens]
- * head_dim is 64 or 128.  A stored value is code * scale. */
+ * head_dim is 64 or 128.  A stored value is code * scale; scales are finite and not
+ * negative, or NaN, as sm_kv8_write leaves them. */
 typedef struct sm_kv8 {
   int8_t* k;
   int8_t* v;
@@ -222,10 +223,25 @@ SM_API int sm_kv8_read(sm_ctx* ctx, const sm_kv8* cache, const int* seq_ids, con
  * to positions 0 .. lens[b] - 1 of slot seq_ids[b] (seq_ids NULL: slot b), with the
  * reference's softmax (MathUtils.FastExp, MathUtils.cs:20-32).  q: row b at
  * q + b * q_stride, [n_heads][head_dim]; out: [B][n_heads * head_dim].
- * 0 <= lens[b] <= max_len <= max_tokens; a row of length 0 gives zeros.  max_len
- * sizes the launch, so a graph captured with it serves every shorter length.
+ * 0 <= lens[b] <= max_len <= max_tokens; a row of length 0 gives zeros.
  * n_heads is a multiple of n_kv, at most 16 q heads per kv head; B is at most 65535.
- * A NaN in q or in a visible scale makes the outputs that depend on it NaN. */
+ *
+ * max_len sizes the launch, so a graph captured with it serves every shorter length, at
+ * a price: the form is chosen, the grid laid out and the workspace taken for max_len.
+ * Where that makes two launches, the workspace is about 4 * g bytes for each row, kv
+ * head and key of max_len (g: q heads per kv head, rounded up to 4, 8 or 16), which the
+ * device's pool keeps afterwards: 1.1 GB for 64 rows, 8 kv heads of 4 q heads and
+ * max_len 131072.  Times: 16 rows of 256 to 2048 keys, 32 / 4 heads of 64: 9.6 us with
+ * max_len 2048 or 4096, 19 us with 32768; 64 rows of 1 to 512 keys, 32 / 8 heads of 128:
+ * 16 us with 512, 39 us with 32768.  Pass the batch's own bound where it is known, and
+ * capture a graph for each of a few bounds.
+ *
+ * Accuracy: q is taken to 22 bits of its head's largest value (and no finer than 2^-143),
+ * products of a weight and a V scale to 2^-24 of the largest V scale that a part of the
+ * keys has; codes are exact, sums exact integers or fp32 (a long shared prefix: runs of
+ * 16 blocks of 128 keys in the tensor cores' fp32 sums, which truncate).  The largest
+ * score's weight is exactly 1.  A NaN in q or in a visible scale makes the outputs that
+ * depend on it NaN, and so does a score outside fp32's range. */
 SM_API int sm_attention_decode_kv8(sm_ctx* ctx, const sm_kv8* cache, const float* q, int64_t q_stride,
                                    const int* seq_ids, const int* lens, int max_len, int B, int n_heads,
                                    float* out);

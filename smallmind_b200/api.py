@@ -366,7 +366,8 @@ class KV8Cache:
     def attention_decode_device(self, q_ptr: int, seq_ptr: int | None, lens_ptr: int, batch: int, n_heads: int,
                                 out_ptr: int, max_len: int | None = None, q_stride: int | None = None):
         """Decode attention, one query row per sequence (sm_attention_decode_kv8).  max_len: an upper
-        bound of this call's lengths (default: the cache's max_tokens)."""
+        bound of this call's lengths (default: the cache's max_tokens), which sizes the launch and its workspace:
+        a close one is faster."""
         if q_stride is None:
             q_stride = n_heads * self.head_dim
         if max_len is None:
@@ -378,7 +379,7 @@ class KV8Cache:
                                 seq_ptr: int | None, lens_ptr: int, batch: int, n_heads: int, out_ptr: int,
                                 max_len: int | None = None, q_stride: int | None = None):
         """Decode attention of a batch that shares the first prefix_len positions of one slot of
-        ``prefix`` (sm_attention_shared_kv8)."""
+        ``prefix`` (sm_attention_shared_kv8).  max_len: as in attention_decode_device."""
         if q_stride is None:
             q_stride = n_heads * self.head_dim
         if max_len is None:

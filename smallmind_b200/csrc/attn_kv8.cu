@@ -828,7 +828,9 @@ constexpr size_t SMEM_MAX = 220 * 1024;
 // Behind a shared prefix, which L2 holds, the other form is attn_kv8_tc.cu, whose five launches take 30 to 40 us at
 // least where head_dim is 128: there the bound is 1056 KB (32 / 8 x 128, prefix of 4096: 16 rows, 1056 KB, 28 us
 // against 40 us; prefix of 1024: 64 rows, 1024 KB, 32 us against 41 us; 32 / 4 x 64, prefix of 4096, 64 rows, 950 KB:
-// 42 us against 32 us).
+// 42 us against 32 us).  Beyond it neither is faster everywhere until 1.4 MB (32 / 8 x 128, 16 rows: 1109 KB 34 us
+// against 55 us, 1356 KB 40 us against 45 us; 16 / 16 x 128, 16 rows over 3000: 1353 KB 44 us against 42 us; 12 / 4 x
+// 128, 64 rows over 3000: 1353 KB 44 us against 38 us) and then the matrix form is (1827 KB 56 us against 45 us).
 struct ClusterPlan {
   int size, cap, warps;
   size_t smem;

@@ -20,12 +20,17 @@
 // CTA's units of one tile make a segment with sums of its own.  The accumulation of O inside the tensor cores
 // truncates: over 111 blocks it was 2e-5 off, so every FLUSH blocks O moves on to fp32 sums in memory.
 //
-// Bound by the tensor cores: at fp32 accuracy a block takes 16 + 32 MMAs (head_dim 128) in the two passes, 64 clocks
-// each.  32 / 8 heads of 128, 256 rows over 32768 keys: max 95 us (82% of the time on the tensor pipe), P V 218 us
-// (72%: P of a block is waited for while both score buffers are taken), prep 33 us (HBM: 67 MB of codes in, 134 MB
-// of tiles out), own keys 45 us, join 10 us.  Four score buffers of 64 keys keep the pipe full, but an MMA of 64
-// columns takes as long as one of 128 (P V 238 us); two halves of the softmax warps that take every other block
-// 230 us; 8 softmax warps instead of 16 the same time.
+// q and P as fp16 pairs hold 22 bits of a row's largest |q| and of the prefix's largest V scale, where fp32 holds 24 of
+// each value; a third half would be half as many MMAs again.
+//
+// Bound by the tensor cores: a block takes 16 + 32 MMAs (head_dim 128) in the two passes, 64 clocks each (counted:
+// the cycles in which the tensor pipe is active, over the MMAs of a CTA, in both passes).  32 / 8 heads of 128, 256
+// rows over 32768 keys, each kernel alone and with cold caches: max 98 us (84 % of the time on the tensor pipe), P V
+// 225 us (70 %: P of a block is waited for while both score buffers are taken), both at an SM clock of 1.60 GHz; prep
+// 34 us (HBM: 67 MB of codes in, 134 MB of tiles out), own keys 50 us, join 12 us; the whole call, whose launches
+// overlap, 377 us.  Tried when P V took 218 us: four score buffers of 64 keys keep the pipe full, but an MMA of 64
+// columns takes as long as one of 128 (238 us); two halves of the softmax warps that take every other block 230 us; 8
+// softmax warps instead of 16 the same time.
 #include <cuda_fp16.h>
 
 #include <algorithm>

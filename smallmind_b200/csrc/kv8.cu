@@ -2,7 +2,9 @@
 //
 // A head's row x[hd] is kept as codes c and one scale s:
 //   s = fl32(max|x| * fl32(1 / 127)),  c = x / s rounded to the nearest integer (ties to even),
-// and read back as fl32(c * s).  The rounding is exact: with q the candidate next to
+// and read back as fl32(c * s).  The scale is a product, within two ulps of the quotient max|x| / 127, because that
+// is what torch makes of x / 127.0 on the GPU (equal on 4 M values): rows quantised there and here have the same
+// scales and codes.  The rounding of the codes is exact: with q the candidate next to
 // x * (1 / s), the remainder r = x - q * s is formed without error by one FMA (q has 7
 // bits and |r| <= ~s, so r fits 24 bits), and q stands unless |r| >= s / 2.  That test
 // fails only for values within an ulp or so of a border, which then take a float64

@@ -1,8 +1,10 @@
 // Integer tensor-core pieces of the 8-bit KV cache's attention (mma.sync m16n8k32).
 //
 // The codes are the A operand as they are.  The fp32 side (q, or the softmax weights) enters as
-// fixed point: three bytes of an integer of up to 24 bits, one MMA per byte, whose exact int32
-// sums are put together in fp32.  So a product keeps fp32 accuracy and no code is converted.
+// fixed point: three bytes of an integer of up to 23 bits, one MMA per byte, whose exact int32
+// sums are put together in fp32.  No code is converted.  A value is off by half a step of 2^-22 (q, relative to its
+// head's largest) or 2^-23 (weights times V scales, to the largest of a warp's keys) at most, where fp32's half step
+// is 2^-24 of the value itself: far below what 8 bits of K and V cost, and a fourth digit would be a third more MMAs.
 #pragma once
 #include <cstdint>
 
