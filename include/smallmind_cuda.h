@@ -241,7 +241,8 @@ SM_API int sm_kv8_read(sm_ctx* ctx, const sm_kv8* cache, const int* seq_ids, con
  * keys has; codes are exact, sums exact integers or fp32 (a long shared prefix: runs of
  * 16 blocks of 128 keys in the tensor cores' fp32 sums, which truncate).  The largest
  * score's weight is exactly 1.  A NaN in q or in a visible scale makes the outputs that
- * depend on it NaN, and so does a score outside fp32's range. */
+ * depend on it NaN; so does a score outside fp32's range, and a key whose scale times the
+ * head's largest |q| is outside it, whatever the score. */
 SM_API int sm_attention_decode_kv8(sm_ctx* ctx, const sm_kv8* cache, const float* q, int64_t q_stride,
                                    const int* seq_ids, const int* lens, int max_len, int B, int n_heads,
                                    float* out);
